@@ -80,6 +80,13 @@ SIGNATURES = {
     "evfly_model_profile_exec_flops": (c_i, [c_p, c_i, C.POINTER(c_d)]),
     "evfly_model_profile_useful_flops": (c_i, [c_p, c_i, C.POINTER(c_d)]),
     "evfly_model_profile_reset": (c_i, [c_p]),
+    "evfly_decay_attention_workspace_bytes": (c_i64, [c_i] * 8),
+    "evfly_decay_attention_forward": (c_i, [c_p] * 7 + [c_i] * 6 + [c_f, c_i, c_p, c_p, c_p, c_i64, c_p]),
+    "evfly_decay_attention_backward": (c_i, [c_p] * 9 + [c_i] * 6 + [c_f, c_i] + [c_p] * 5 + [c_i64, c_p]),
+    "evfly_block_norm_workspace_bytes": (c_i64, [c_i64, c_i, c_i64, c_i]),
+    "evfly_block_norm_forward": (c_i, [c_p, c_p, c_p, c_i64, c_i, c_i, c_p, c_i, c_p, c_p, c_i, c_p, c_p, c_f, c_i64, c_i, c_i, c_p, c_p, c_p]),
+    "evfly_block_norm_backward": (c_i, [c_p, c_p, c_p, c_i64, c_i, c_i, c_p, c_i, c_p, c_p, c_i, c_p, c_p, c_f, c_p, c_p, c_i64, c_i, c_i]
+                                  + [c_p] * 9 + [c_i64, c_p]),
     "evfly_op_conv2d_nhwc": (c_i, [c_p, c_i, c_i, c_i, c_i, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i,
                                    c_p, c_p, c_i, c_p]),
     "evfly_op_pool2d_nhwc": (c_i, [c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_p]),

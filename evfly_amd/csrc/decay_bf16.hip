@@ -1,0 +1,8 @@
+// Decay attention, bf16 tokens (v_mfma_f32_16x16x32_bf16, fp32 accumulate and state).
+#include <atomic>
+
+#include "decay_kernel.h"
+
+namespace evfly {
+int decay_pass_bf16(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st) { return decay::launch_all<bf16_t>(p, pl, vec, st); }
+}  // namespace evfly

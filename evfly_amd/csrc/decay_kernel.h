@@ -1,0 +1,461 @@
+// The chunked kernel of decay attention for one element type (included by decay_f32.hip and decay_bf16.hip).
+//
+// A chunk of 64 tokens (local index i = t - t0) against the state S that the chunks before it left:
+//     out_i = f_out e^{g (i + o)} a_i S  +  sum_{j <= i} f_intra e^{g (i - j)} (a_i . b_j) c_j
+//     S'    = e^{g cnt} S  +  sum_j f_upd e^{g (cnt - j - o)} b_j c_j^T                 cnt tokens in the chunk; o = 1 forwards, 0 backwards
+// Every exponent is a whole number of steps in [0, 64], so one table of 65 powers per head serves all of them and no weight is the quotient of two
+// others. All four products run on 16x16 MFMAs with token columns: P^T = b a^T leaves, in a lane, pair weights of one token i against
+// four neighbouring j, which is the operand layout of out^T = c^T P^T -- the pair products never leave registers.
+//
+// Work: one block of four waves per (stream, head, tile of DC columns of c, segment); wave w owns the chunk's tokens 16 w .. 16 w + 15
+// of the output and a share of the state's a-rows. The a rows go from memory to the wave's registers, b and c through LDS (read as rows for P, as
+// columns for the other two products), S lives in the accumulators and is copied to LDS once per chunk as an operand of a_i S. The next chunk's rows
+// are in flight during the products.
+#pragma once
+#include "bf16.h"
+#include "decay.h"
+
+namespace evfly {
+namespace decay {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// Element-type side: a fragment is 16 bytes per lane = KB / 4 values of the summed index (KB per MFMA step over the four lane groups).
+template <typename T> struct Mm;
+
+template <> struct Mm<float> {
+    static constexpr int KB = 16;       // values of the summed index per fragment
+    static constexpr int TILES = 1;     // 16-row tiles of it
+    static constexpr int NU = 1;        // parts of a weighted operand (exact)
+    static constexpr int NP = 1;        // parts of P and S as operands
+    typedef f32x4 frag;
+    __device__ static __forceinline__ frag load(const char *lds) { return *reinterpret_cast<const frag *>(lds); }
+    __device__ static __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+    // column `col` of rows 16 kb + 4 g .. + 3 of a row-major tile (row stride rsb bytes)
+    __device__ static __forceinline__ frag load_col(const char *tile, int rsb, int kb, int g, int col) {
+        frag f;
+        const char *p = tile + (16 * kb + 4 * g) * rsb + col * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const float *>(p + i * rsb);
+        return f;
+    }
+    __device__ static __forceinline__ void weigh(frag b, const float *w, frag (&o)[NU]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[0][i] = b[i] * w[i];
+    }
+    __device__ static __forceinline__ void split(const f32x4 *acc, frag (&o)[NP]) { o[0] = acc[0]; }
+    __device__ static __forceinline__ void put_state(char *p, int, f32x4 s) { *reinterpret_cast<f32x4 *>(p) = s; }
+};
+
+// hi + mid + lo of an fp32 value as bf16 (8 + 8 + 8 significant bits, each part the rounding of what the parts before it left): two parts carry 2^-17 of
+// the value, three all of its 24 bits. A part that rounds to infinity, or a value that is not finite, leaves nothing to the next one.
+__device__ __forceinline__ float left_over(float x, float hi) {
+    const float r = x - hi;
+    return fabsf(hi) < INFINITY ? r : 0.f;
+}
+
+template <> struct Mm<bf16_t> {
+    static constexpr int KB = 32;
+    static constexpr int TILES = 2;
+    static constexpr int NU = 3;        // the fp32 state is an output: its update keeps all 24 bits of weight * value
+    static constexpr int NP = 2;        // P and S meet bf16 outputs: 2^-17 of each, far below the output's own rounding of 2^-9
+    typedef bf16x8 frag;
+    union U { uint4 u; frag f; i16x4 h[2]; };
+    __device__ static __forceinline__ frag load(const char *lds) { return *reinterpret_cast<const frag *>(lds); }
+    __device__ static __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    // summed index in the order of two accumulator tiles: values 0..3 = rows 32 kb + 4 g + e, values 4..7 = rows 32 kb + 16 + 4 g + e. The transposed LDS
+    // read takes, for 16 lanes, the addresses of four rows of four 8-byte pieces and hands lane l column l of the four rows.
+    __device__ static __forceinline__ frag load_col(const char *tile, int rsb, int kb, int g, int col) {
+        const int l = col & 15, c0 = col & ~15;
+        const char *p = tile + (32 * kb + 4 * g + (l >> 2)) * rsb + (c0 + 4 * (l & 3)) * 2;
+        U r;
+        typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+        r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(p));
+        r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(p + 16 * rsb));
+        return r.f;
+    }
+    __device__ static __forceinline__ void parts(const float (&x)[8], frag *o, int n) {
+        float r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
+        for (int k = 0; k < n; ++k) {
+            unsigned w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = pack_bf2(r[2 * e], r[2 * e + 1]);
+                if (k + 1 < n) {
+                    r[2 * e] = left_over(r[2 * e], bf_lo(w[e]));
+                    r[2 * e + 1] = left_over(r[2 * e + 1], bf_hi(w[e]));
+                }
+            }
+            U u;
+            u.u = make_uint4(w[0], w[1], w[2], w[3]);
+            o[k] = u.f;
+        }
+    }
+    __device__ static __forceinline__ void weigh(frag b, const float *w, frag (&o)[NU]) {
+        U u;
+        u.f = b;
+        const unsigned d[4] = {u.u.x, u.u.y, u.u.z, u.u.w};
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[2 * e] = bf_lo(d[e]) * w[2 * e];
+            x[2 * e + 1] = bf_hi(d[e]) * w[2 * e + 1];
+        }
+        parts(x, o, NU);
+    }
+    __device__ static __forceinline__ void split(const f32x4 *acc, frag (&o)[NP]) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[e] = acc[0][e]; x[4 + e] = acc[1][e]; }
+        parts(x, o, NP);
+    }
+    // four neighbouring a-values of one column of S, as two bf16 planes
+    __device__ static __forceinline__ void put_state(char *p, int plane, f32x4 s) {
+        const unsigned h0 = pack_bf2(s[0], s[1]), h1 = pack_bf2(s[2], s[3]);
+        *reinterpret_cast<uint2 *>(p) = make_uint2(h0, h1);
+        *reinterpret_cast<uint2 *>(p + plane) = make_uint2(pack_bf2(left_over(s[0], bf_lo(h0)), left_over(s[1], bf_hi(h0))),
+                                                           pack_bf2(left_over(s[2], bf_lo(h1)), left_over(s[3], bf_hi(h1))));
+    }
+};
+
+// 16 bytes of a token row from column `col` on, zeros behind column d. VEC: rows are 16-byte aligned and d is a multiple of the vector.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load16(const T *row, int col, int d) {
+    constexpr int V = 16 / sizeof(T);
+    if (VEC) return col < d ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0, 0, 0, 0);
+    union { T v[V]; uint4 u; } r;
+#pragma unroll
+    for (int e = 0; e < V; ++e) r.v[e] = col + e < d ? row[col + e] : T(0);
+    return r.u;
+}
+
+template <typename T, int DA, int DC> struct Lds {
+    static constexpr int RB = DA * (int)sizeof(T) + 16;        // row strides in bytes: 16 more than the row, so that 16 rows read at one column
+    static constexpr int RC = DC * (int)sizeof(T) + 16;        // spread over the banks
+    static constexpr int RS = DA * (int)sizeof(T) + 16;
+    static constexpr int PW = 0, B = 512, C = B + DECAY_CHUNK * RB, S = C + DECAY_CHUNK * RC;
+    static constexpr int PLANE = DC * RS;
+    static constexpr int BYTES = S + PLANE * Mm<T>::NP;
+};
+
+// STATE: the segment's own state only (no output), for the sequences that are split into segments.
+template <typename T, int DA, int DC, bool VEC, bool STATE>
+__global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
+    typedef Mm<T> M;
+    typedef typename M::frag frag;
+    typedef Lds<T, DA, DC> L;
+    constexpr int C = DECAY_CHUNK, V = 16 / sizeof(T);
+    constexpr int KA = DA / M::KB;                   // fragments along a
+    constexpr int KS = C / M::KB;                    // fragments along the chunk
+    constexpr int NC = DC / 16;                      // 16-column tiles of c
+    constexpr int NA = DA >= 64 ? DA / 64 : 1;       // the wave's share of the state: NA a-tiles by NCW c-tiles
+    constexpr int NCW = DA >= 64 ? NC : NC / 2;
+    constexpr int NB = C * DA / V / 256, NV = C * DC / V / 256;      // 16-byte pieces per thread of a chunk of b and c
+    static_assert(NB >= 1 && NV >= 1, "a chunk is at least one piece per thread");
+    extern __shared__ __align__(16) char lds[];
+    float *const pw = reinterpret_cast<float *>(lds + L::PW);
+
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
+    // blocks of one XCD (block index mod 8) take neighbouring work: the heads of a token share cache lines, shared heads and column tiles share rows
+    const int total = gridDim.x, q8 = total / kNumXCD, r8 = total % kNumXCD, xcd = blockIdx.x % kNumXCD;
+    int id = xcd * q8 + min(xcd, r8) + blockIdx.x / kNumXCD;
+    const int nseg = STATE ? p.nseg - 1 : p.nseg;
+    const int c0 = (id % ndc) * DC; id /= ndc;
+    const int h = id % p.H; id /= p.H;
+    const int seg = id % nseg;
+    const int n = id / nseg;
+
+    const int len = p.lengths ? min(max(p.lengths[n], 0), p.T) : p.T;
+    const int u_lo = seg * p.seg_len, u_hi = min(u_lo + p.seg_len, p.T), u_end = min(u_hi, len);
+    const int dcw = min(p.dc - c0, DC);              // columns of this tile
+    const int o = p.rev ? 0 : 1;
+    const T *const ap = static_cast<const T *>(p.a) + n * p.as[0] + (h / p.ra) * p.as[2];
+    const T *const bp = static_cast<const T *>(p.b) + n * p.bs[0] + (h / p.rb) * p.bs[2];
+    const T *const cp = static_cast<const T *>(p.c) + n * p.cs[0] + (h / p.rc) * p.cs[2] + c0;
+    const int64_t st_base = ((int64_t)n * p.H + h) * p.da * p.dc;
+    const int64_t ot = (int64_t)p.H * p.dc;          // output elements per token
+    const int64_t ob = ((int64_t)n * p.T * p.H + h) * p.dc + c0;
+
+    if (tid <= C) pw[tid] = tid == 0 ? 1.f : expf(p.log_decay[h] * (float)tid);
+
+    // ---- the state: rows a = 16 (a-tile) + 4 g + i, column c = 16 (c-tile) + l
+    const int a_t0 = DA >= 64 ? w * NA : w & 1, c_t0 = DA >= 64 ? 0 : (w >> 1) * NCW;
+    f32x4 S[NA][NCW];
+    const int tile_id = ((n * p.H + h) * ndc + c0 / DC);
+    float *const slots = p.seg + (int64_t)tile_id * p.nseg * (DA * DC);      // (nseg > 1)
+#pragma unroll
+    for (int x = 0; x < NA; ++x)
+#pragma unroll
+        for (int y = 0; y < NCW; ++y) {
+            if (!STATE && p.nseg > 1) {
+                S[x][y] = *reinterpret_cast<const f32x4 *>(slots + (int64_t)seg * (DA * DC) + ((x * NCW + y) * 256 + tid) * 4);
+            } else {
+                const int a = 16 * (a_t0 + x) + 4 * g, c = 16 * (c_t0 + y) + l;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    S[x][y][i] = !STATE && p.s_in && a + i < p.da && c < dcw ? p.s_in[st_base + (a + i) * p.s_a + (c0 + c) * p.s_c] : 0.f;
+            }
+        }
+
+    uint4 rb[NB], rc[NV];
+    frag fa[KA], fa_next[KA];
+    auto fetch = [&](int u0) {
+#pragma unroll
+        for (int x = 0; x < NB; ++x) {
+            const int v = x * 256 + tid, r = v / (DA / V), col = v % (DA / V) * V, u = u0 + r;
+            rb[x] = make_uint4(0, 0, 0, 0);
+            if (u < u_end) rb[x] = load16<T, VEC>(bp + (int64_t)(p.rev ? len - 1 - u : u) * p.bs[1], col, p.da);
+        }
+#pragma unroll
+        for (int x = 0; x < NV; ++x) {
+            const int v = x * 256 + tid, r = v / (DC / V), col = v % (DC / V) * V, u = u0 + r;
+            rc[x] = make_uint4(0, 0, 0, 0);
+            if (u < u_end) rc[x] = load16<T, VEC>(cp + (int64_t)(p.rev ? len - 1 - u : u) * p.cs[1], col, dcw);
+        }
+        if (!STATE) {
+            const int u = u0 + 16 * w + l;
+            const T *row = ap + (int64_t)(p.rev ? len - 1 - u : u) * p.as[1];
+#pragma unroll
+            for (int k = 0; k < KA; ++k) {
+                union { uint4 u4; frag f; } t;
+                t.u4 = make_uint4(0, 0, 0, 0);
+                if (u < u_end) t.u4 = load16<T, VEC>(row, k * M::KB + g * V, p.da);
+                fa_next[k] = t.f;
+            }
+        }
+    };
+    if (u_lo < u_end) fetch(u_lo);
+    __syncthreads();
+
+    // ---- weights that are the same in every chunk: pairs of token i = 16 w + l with j = 16 st + 4 g + e, and the update of a full chunk
+    float wp[4][4], wu[4][4];
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int j = 16 * st + 4 * g + e, d = 16 * w + l - j;
+            wp[st][e] = d >= 0 ? p.f_intra * pw[max(d, 0)] : 0.f;
+            wu[st][e] = p.f_upd * pw[C - j - o];
+        }
+    const float w_out = p.f_out * pw[16 * w + l + o];
+
+    for (int u0 = u_lo; u0 < u_end; u0 += C) {
+        const int cnt = min(C, u_end - u0);
+        if (u0 > u_lo) __syncthreads();              // the products of the chunk before have read their tiles
+#pragma unroll
+        for (int x = 0; x < NB; ++x) {
+            const int v = x * 256 + tid;
+            *reinterpret_cast<uint4 *>(lds + L::B + v / (DA / V) * L::RB + v % (DA / V) * 16) = rb[x];
+        }
+#pragma unroll
+        for (int x = 0; x < NV; ++x) {
+            const int v = x * 256 + tid;
+            *reinterpret_cast<uint4 *>(lds + L::C + v / (DC / V) * L::RC + v % (DC / V) * 16) = rc[x];
+        }
+        if (!STATE) {
+#pragma unroll
+            for (int x = 0; x < NA; ++x)
+#pragma unroll
+                for (int y = 0; y < NCW; ++y)
+                    M::put_state(lds + L::S + (16 * (c_t0 + y) + l) * L::RS + (16 * (a_t0 + x) + 4 * g) * (int)sizeof(T), L::PLANE, S[x][y]);
+#pragma unroll
+            for (int k = 0; k < KA; ++k) fa[k] = fa_next[k];
+        }
+        __syncthreads();
+        if (u0 + C < u_end) fetch(u0 + C);
+
+        if (!STATE) {
+            // ---- P^T tiles of this wave's tokens (j-tiles up to its own), weighted, as operand parts
+            frag P[KS][M::NP];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks * M::TILES > w) continue;
+                f32x4 acc[M::TILES];
+#pragma unroll
+                for (int x = 0; x < M::TILES; ++x) {
+                    const int st = ks * M::TILES + x;
+                    acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (st > w) continue;
+#pragma unroll
+                    for (int k = 0; k < KA; ++k)
+                        acc[x] = M::mma(M::load(lds + L::B + (16 * st + l) * L::RB + k * 64 + g * 16), fa[k], acc[x]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)          // a later token's product is dropped, not multiplied by zero
+                        acc[x][e] = st < w || 4 * g + e <= l ? acc[x][e] * wp[st][e] : 0.f;
+                }
+                M::split(acc, P[ks]);
+            }
+            // ---- out^T = w_out S^T a^T + c^T P^T
+            const int u = u0 + 16 * w + l;
+            const int64_t oi = ob + (int64_t)(p.rev ? len - 1 - u : u) * ot;
+#pragma unroll
+            for (int y = 0; y < NC; ++y) {
+                f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KA; ++k)
+#pragma unroll
+                    for (int x = 0; x < M::NP; ++x)
+                        acc = M::mma(M::load(lds + L::S + x * L::PLANE + (16 * y + l) * L::RS + k * 64 + g * 16), fa[k], acc);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] *= w_out;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (ks * M::TILES > w) continue;
+                    const frag fc = M::load_col(lds + L::C, L::RC, ks, g, 16 * y + l);
+#pragma unroll
+                    for (int x = 0; x < M::NP; ++x) acc = M::mma(fc, P[ks][x], acc);
+                }
+                const int c = 16 * y + 4 * g;
+                if (u < u_end && c < dcw) {
+                    if (p.out_f32) {
+                        float *d = static_cast<float *>(p.out) + oi + c;
+                        if (VEC) *reinterpret_cast<f32x4 *>(d) = acc;
+                        else
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (c + e < dcw) d[e] = acc[e];
+                    } else {
+                        T *d = static_cast<T *>(p.out) + oi + c;
+                        if (sizeof(T) == 4) {
+                            if (VEC) *reinterpret_cast<f32x4 *>(d) = acc;
+                            else
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (c + e < dcw) Elem<T>::st1(d + e, acc[e]);
+                        } else {
+                            if (VEC) *reinterpret_cast<uint2 *>(d) = make_uint2(pack_bf2(acc[0], acc[1]), pack_bf2(acc[2], acc[3]));
+                            else
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (c + e < dcw) Elem<T>::st1(d + e, acc[e]);
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- S = e^{g cnt} S + (w b)^T c
+        if (cnt < C)
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wu[st][e] = p.f_upd * pw[max(cnt - (16 * st + 4 * g + e) - o, 0)];      // (rows behind cnt are zero)
+        const float keep = pw[cnt];
+#pragma unroll
+        for (int x = 0; x < NA; ++x)
+#pragma unroll
+            for (int y = 0; y < NCW; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[x][y][e] *= keep;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            frag fb[NA][M::NU];
+#pragma unroll
+            for (int x = 0; x < NA; ++x)
+                M::weigh(M::load_col(lds + L::B, L::RB, ks, g, 16 * (a_t0 + x) + l), &wu[ks * M::TILES][0], fb[x]);
+#pragma unroll
+            for (int y = 0; y < NCW; ++y) {
+                const frag fc = M::load_col(lds + L::C, L::RC, ks, g, 16 * (c_t0 + y) + l);
+#pragma unroll
+                for (int x = 0; x < NA; ++x)
+#pragma unroll
+                    for (int z = 0; z < M::NU; ++z) S[x][y] = M::mma(fb[x][z], fc, S[x][y]);
+            }
+        }
+    }
+
+    if (STATE) {
+#pragma unroll
+        for (int x = 0; x < NA; ++x)
+#pragma unroll
+            for (int y = 0; y < NCW; ++y)
+                *reinterpret_cast<f32x4 *>(slots + (int64_t)(seg + 1) * (DA * DC) + ((x * NCW + y) * 256 + tid) * 4) = S[x][y];
+        return;
+    }
+    // ---- rows behind the sequence are zero; the last segment ends with the state behind the whole sequence
+    for (int64_t i = tid; i < (int64_t)max(0, u_hi - max(u_lo, len)) * dcw; i += 256) {
+        const int64_t at = ob + (max(u_lo, len) + i / dcw) * ot + i % dcw;
+        if (p.out_f32) static_cast<float *>(p.out)[at] = 0.f;
+        else static_cast<T *>(p.out)[at] = T(0);
+    }
+    if (p.s_fin && seg == p.nseg - 1)
+#pragma unroll
+        for (int x = 0; x < NA; ++x)
+#pragma unroll
+            for (int y = 0; y < NCW; ++y) {
+                const int a = 16 * (a_t0 + x) + 4 * g, c = 16 * (c_t0 + y) + l;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (a + i < p.da && c < dcw) p.s_fin[st_base + (a + i) * p.s_a + (c0 + c) * p.s_c] = S[x][y][i];
+            }
+}
+
+// States the segments start from: slot s + 1 holds segment s's own state, slot s receives
+//     start_{s+1} = e^{g cnt_s} start_s + own_s,    start_0 = s_in
+// (start_0 as well: the last segment may write its final state over s_in while the first one runs). One thread per four accumulator values
+// of k_decay_chunk, the same place in every slot.
+template <int DA, int DC> __global__ __launch_bounds__(256) void k_decay_scan(DecayPass p, int ndc) {
+    constexpr int NA = DA >= 64 ? DA / 64 : 1, NC = DC / 16, NCW = DA >= 64 ? NC : NC / 2;
+    const int vec = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int tile = blockIdx.x, nh = tile / ndc, c0 = tile % ndc * DC, n = nh / p.H, h = nh % p.H;
+    const int len = p.lengths ? min(max(p.lengths[n], 0), p.T) : p.T;
+    const float gl = p.log_decay[h];
+    const int x = vec / NCW, y = vec % NCW;
+    const int a = 16 * ((DA >= 64 ? w * NA : w & 1) + x) + 4 * g, c = 16 * ((DA >= 64 ? 0 : (w >> 1) * NCW) + y) + l;
+    f32x4 S = {0.f, 0.f, 0.f, 0.f};
+    if (p.s_in)
+        for (int i = 0; i < 4; ++i)
+            if (a + i < p.da && c0 + c < p.dc) S[i] = p.s_in[(int64_t)nh * p.da * p.dc + (a + i) * p.s_a + (c0 + c) * p.s_c];
+    f32x4 *slot = reinterpret_cast<f32x4 *>(p.seg) + (int64_t)tile * p.nseg * (DA * DC / 4) + vec * 256 + tid;
+    slot[0] = S;
+#pragma unroll 8
+    for (int s = 1; s < p.nseg; ++s) {
+        const int cnt = min(max(len - (s - 1) * p.seg_len, 0), p.seg_len);
+        const float keep = cnt == 0 ? 1.f : expf(gl * (float)cnt);
+        const f32x4 own = slot[(int64_t)s * (DA * DC / 4)];
+        for (int i = 0; i < 4; ++i) S[i] = keep * S[i] + own[i];
+        slot[(int64_t)s * (DA * DC / 4)] = S;
+    }
+}
+
+template <typename T, int DA, int DC, bool VEC> int launch(const DecayPass &p, const DecayPlan &pl, hipStream_t st) {
+    typedef Lds<T, DA, DC> L;
+    static_assert(L::BYTES <= kMaxLds, "LDS of one CU");
+    const int64_t tiles = (int64_t)p.n * p.H * pl.ndc;
+    EVFLY_REQUIRE(tiles * pl.nseg <= INT32_MAX, "decay_attention: %lld tiles of work", (long long)(tiles * pl.nseg));
+    static std::atomic<bool> attr_set[64];
+    int dev = 0;
+    EVFLY_HIP(hipGetDevice(&dev));
+    EVFLY_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+        EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_decay_chunk<T, DA, DC, VEC, false>), hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES));
+        EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_decay_chunk<T, DA, DC, VEC, true>), hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES));
+        attr_set[dev].store(true, std::memory_order_release);
+    }
+    if (pl.nseg > 1) {
+        hipLaunchKernelGGL((k_decay_chunk<T, DA, DC, VEC, true>), dim3((unsigned)(tiles * (pl.nseg - 1))), dim3(256), L::BYTES, st, p, pl.ndc);
+        hipLaunchKernelGGL((k_decay_scan<DA, DC>), dim3((unsigned)tiles, DA * DC / 1024), dim3(256), 0, st, p, pl.ndc);
+    }
+    hipLaunchKernelGGL((k_decay_chunk<T, DA, DC, VEC, false>), dim3((unsigned)(tiles * pl.nseg)), dim3(256), L::BYTES, st, p, pl.ndc);
+    EVFLY_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T, int DA, int DC> int launch_v(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st) {
+    return vec ? launch<T, DA, DC, true>(p, pl, st) : launch<T, DA, DC, false>(p, pl, st);
+}
+template <typename T> int launch_all(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st) {
+    if (pl.DC == 32) return pl.DA == 32 ? launch_v<T, 32, 32>(p, pl, vec, st) : pl.DA == 64 ? launch_v<T, 64, 32>(p, pl, vec, st) : launch_v<T, 128, 32>(p, pl, vec, st);
+    return pl.DA == 32 ? launch_v<T, 32, 64>(p, pl, vec, st) : pl.DA == 64 ? launch_v<T, 64, 64>(p, pl, vec, st) : launch_v<T, 128, 64>(p, pl, vec, st);
+}
+
+}  // namespace decay
+}  // namespace evfly

@@ -338,6 +338,75 @@ int evfly_model_profile_useful_flops(evfly_model *m, int i, double *useful_flops
 int evfly_model_profile_reset(evfly_model *m);
 
 /* ------------------------------------------------------------------------------------------
+ * Temporal operators: a mixer over the windows of many streams and the norm / gate / residual around it. No reference
+ * counterpart; they stand beside evfly_convlstm_forward (a state carried per stream) and the block halves of
+ * evfly_vit_block_forward (attention, LayerNorm(x + f)). dtype EVFLY_DTYPE_F32 or EVFLY_DTYPE_BF16 = type of the token
+ * tensors (fp32, or bf16 raw bits); sums, statistics and states are fp32 in both.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Decay attention: linear attention with one constant decay per head,
+ *     S_t = exp(log_decay[h]) * S_{t-1} + k_t v_t^T           (dk x dv per stream and head)
+ *     out_t = scale * q_t S_t
+ * q (n_streams, tokens, heads, dk), k (n_streams, tokens, kv_heads, dk), v (n_streams, tokens, kv_heads, dv), out
+ * (n_streams, tokens, heads, dv); heads is a multiple of kv_heads and query head h reads key / value head
+ * h / (heads / kv_heads). 1 <= dk, dv <= EVFLY_DECAY_MAX_DIM. strides_host: nine element strides on the HOST (stream, token, head of q, then of
+ * k, then of v; the last dimension is contiguous), NULL = contiguous tensors; out is contiguous.
+ * log_decay (heads) fp32: 0 keeps everything, -inf keeps nothing (out_t = scale * (q_t . k_t) v_t); positive values grow and are
+ * computed as they stand.
+ * state_in (n_streams, heads, dk, dv) fp32 or NULL = zeros; state_out the same, or NULL = not wanted; they may be the same buffer.
+ * lengths (n_streams) int32 or NULL: stream i has lengths[i] tokens (taken into [0, tokens]); what q, k, v hold behind them is
+ * not read, out is zero there, and state_out is the state after the stream's last token (a stream of no tokens keeps its state).
+ * Inside a sequence a non-finite k or v reaches every later token, and may reach the earlier tokens of its own group of 64.
+ * Up to EVFLY_DECAY_STEP_TOKENS tokens (one window per stream is the serving form) run as the recurrence with the state in registers and need
+ * no workspace, longer ones in chunks of 64 on the matrix cores. workspace: at least
+ * evfly_decay_attention_workspace_bytes(..., backward = 0) bytes (may be 0: workspace NULL), 16-byte aligned; one per call in
+ * flight. What it holds before the call does not matter. */
+#define EVFLY_DECAY_MAX_DIM 128
+#define EVFLY_DECAY_STEP_TOKENS 16
+int64_t evfly_decay_attention_workspace_bytes(int n_streams, int tokens, int heads, int kv_heads, int dk, int dv, int dtype,
+                                              int backward);
+int evfly_decay_attention_forward(const void *q, const void *k, const void *v, const int64_t *strides_host,
+                                  const float *log_decay, const float *state_in, const int32_t *lengths, int n_streams,
+                                  int tokens, int heads, int kv_heads, int dk, int dv, float scale, int dtype, void *out,
+                                  float *state_out, void *workspace, int64_t workspace_bytes, void *stream);
+/* Its gradients: d_out (n_streams, tokens, heads, dv) and d_state_out (n_streams, heads, dk, dv) fp32 or NULL = zeros come in;
+ * dq, dk, dv (contiguous, shaped like q, k, v; the sum over the query heads that share a key / value head) and d_state_in (fp32, may be NULL) go
+ * out. d_out is not read and dq, dk, dv are zero behind a stream's length. log_decay is a constant: it has no gradient. */
+int evfly_decay_attention_backward(const void *q, const void *k, const void *v, const int64_t *strides_host,
+                                   const float *log_decay, const float *state_in, const int32_t *lengths, const void *d_out,
+                                   const float *d_state_out, int n_streams, int tokens, int heads, int kv_heads, int dk, int dv,
+                                   float scale, int dtype, void *dq, void *dk_out, void *dv_out, float *d_state_in, void *workspace,
+                                   int64_t workspace_bytes, void *stream);
+
+/* Block norm: the norms behind and in front of a block's sub-layer with its gate and residual scale in one pass per token row,
+ *     y = res_scale * x + act(gate) * norm_post(f)            h = norm_pre(y)
+ * f, x, y, h (rows, channels) contiguous; 1 <= channels <= EVFLY_BLOCK_NORM_MAX_CHANNELS. x NULL: no residual. res_scale (channels) fp32 or
+ * NULL = 1. norm kinds: EVFLY_NORM_NONE (the identity; pre NONE: h is not written and may be NULL), EVFLY_NORM_LAYER (mean and biased variance), EVFLY_NORM_RMS; weight
+ * (channels) fp32 or NULL = 1, bias (channels) fp32 or NULL = 0, eps inside the square root. h is formed from y before y is rounded.
+ * gate NULL: none; else (rows / rows_per_gate, channels), row r reads gate row r / rows_per_gate (1: a gate per token; the
+ * tokens of a stream: one per stream; rows: one vector), in the tokens' type, or fp32 with gate_f32 != 0; gate_act EVFLY_ACT_NONE / _TANH /
+ * _SIGMOID. evfly's own block tail LayerNorm(x + f) is post NONE, pre LAYER, no gate. */
+#define EVFLY_BLOCK_NORM_MAX_CHANNELS 8192
+#define EVFLY_NORM_NONE 0
+#define EVFLY_NORM_LAYER 1
+#define EVFLY_NORM_RMS 2
+int evfly_block_norm_forward(const void *f, const void *x, const void *gate, int64_t rows_per_gate, int gate_f32, int gate_act,
+                             const float *res_scale, int post_kind, const float *post_weight, const float *post_bias,
+                             int pre_kind, const float *pre_weight, const float *pre_bias, float eps, int64_t rows, int channels,
+                             int dtype, void *y, void *h, void *stream);
+/* Its gradients from the forward's inputs (statistics are recomputed: the rows are read anyway). dy, dh (rows, channels); dh is
+ * read only with a pre norm, and NULL = zeros for either. df is required, dx may be NULL (no residual). d_gate: shaped like gate, in its type. d_res_scale, d_post_weight, d_post_bias,
+ * d_pre_weight, d_pre_bias (channels) fp32. Every one of them except df may be NULL = not wanted. Column sums are added in a fixed order
+ * (no atomics): the same call gives the same bits. workspace: at least evfly_block_norm_workspace_bytes(...) bytes, 16-byte aligned. */
+int64_t evfly_block_norm_workspace_bytes(int64_t rows, int channels, int64_t rows_per_gate, int dtype);
+int evfly_block_norm_backward(const void *f, const void *x, const void *gate, int64_t rows_per_gate, int gate_f32, int gate_act,
+                              const float *res_scale, int post_kind, const float *post_weight, const float *post_bias,
+                              int pre_kind, const float *pre_weight, const float *pre_bias, float eps, const void *dy, const void *dh,
+                              int64_t rows, int channels, int dtype, void *df, void *dx, void *d_gate, float *d_res_scale,
+                              float *d_post_weight, float *d_post_bias, float *d_pre_weight, float *d_pre_bias, void *workspace,
+                              int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * Single-operator entry points (kernel-level parity tests; same kernels the models launch)
  * ---------------------------------------------------------------------------------------- */
 
