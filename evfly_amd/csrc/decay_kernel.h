@@ -54,12 +54,7 @@ template <> struct Mm<float> {
 };
 
 // hi + mid + lo of an fp32 value as bf16 (8 + 8 + 8 significant bits, each part the rounding of what the parts before it left): two parts carry 2^-17 of
-// the value, three all of its 24 bits. A part that rounds to infinity, or a value that is not finite, leaves nothing to the next one.
-__device__ __forceinline__ float left_over(float x, float hi) {
-    const float r = x - hi;
-    return fabsf(hi) < INFINITY ? r : 0.f;
-}
-
+// the value, three all of its 24 bits. An infinity (or a value within 2^-9 of the largest float) leaves NaN to the next part.
 template <> struct Mm<bf16_t> {
     static constexpr int KB = 32;
     static constexpr int TILES = 2;
@@ -91,8 +86,8 @@ template <> struct Mm<bf16_t> {
             for (int e = 0; e < 4; ++e) {
                 w[e] = pack_bf2(r[2 * e], r[2 * e + 1]);
                 if (k + 1 < n) {
-                    r[2 * e] = left_over(r[2 * e], bf_lo(w[e]));
-                    r[2 * e + 1] = left_over(r[2 * e + 1], bf_hi(w[e]));
+                    r[2 * e] -= bf_lo(w[e]);
+                    r[2 * e + 1] -= bf_hi(w[e]);
                 }
             }
             U u;
@@ -122,18 +117,17 @@ template <> struct Mm<bf16_t> {
     __device__ static __forceinline__ void put_state(char *p, int plane, f32x4 s) {
         const unsigned h0 = pack_bf2(s[0], s[1]), h1 = pack_bf2(s[2], s[3]);
         *reinterpret_cast<uint2 *>(p) = make_uint2(h0, h1);
-        *reinterpret_cast<uint2 *>(p + plane) = make_uint2(pack_bf2(left_over(s[0], bf_lo(h0)), left_over(s[1], bf_hi(h0))),
-                                                           pack_bf2(left_over(s[2], bf_lo(h1)), left_over(s[3], bf_hi(h1))));
+        *reinterpret_cast<uint2 *>(p + plane) = make_uint2(pack_bf2(s[0] - bf_lo(h0), s[1] - bf_hi(h0)), pack_bf2(s[2] - bf_lo(h1), s[3] - bf_hi(h1)));
     }
 };
 
-// 16 bytes of a token row from column `col` on, zeros behind column d. VEC: rows are 16-byte aligned and d is a multiple of the vector.
-template <typename T, bool VEC> __device__ __forceinline__ uint4 load16(const T *row, int col, int d) {
+// 16 bytes of a token row of which `n` values are left (n <= 0: none), zeros behind them. VEC: rows are 16-byte aligned and end with a whole piece.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load16(const T *at, int n) {
     constexpr int V = 16 / sizeof(T);
-    if (VEC) return col < d ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0, 0, 0, 0);
+    if (VEC) return n > 0 ? *reinterpret_cast<const uint4 *>(at) : make_uint4(0, 0, 0, 0);
     union { T v[V]; uint4 u; } r;
 #pragma unroll
-    for (int e = 0; e < V; ++e) r.v[e] = col + e < d ? row[col + e] : T(0);
+    for (int e = 0; e < V; ++e) r.v[e] = e < n ? at[e] : T(0);
     return r.u;
 }
 
@@ -141,14 +135,20 @@ template <typename T, int DA, int DC> struct Lds {
     static constexpr int RB = DA * (int)sizeof(T) + 16;        // row strides in bytes: 16 more than the row, so that 16 rows read at one column
     static constexpr int RC = DC * (int)sizeof(T) + 16;        // spread over the banks
     static constexpr int RS = DA * (int)sizeof(T) + 16;
-    static constexpr int PW = 0, B = 512, C = B + DECAY_CHUNK * RB, S = C + DECAY_CHUNK * RC;
+    static constexpr int PW = 0, UW = 272, B = 1024, C = B + DECAY_CHUNK * RB, S = C + DECAY_CHUNK * RC;
     static constexpr int PLANE = DC * RS;
     static constexpr int BYTES = S + PLANE * Mm<T>::NP;
 };
 
+// Blocks that share a CU: as many as LDS and registers hold without spills.
+template <typename T, int DA, int DC> constexpr int blocks_per_cu() {
+    constexpr int regs = sizeof(T) == 4 ? (DA == 128 ? 2 : DA == 64 ? 3 : 4) : DA == 128 ? 3 : 4, fit = kMaxLds / Lds<T, DA, DC>::BYTES;
+    return fit < regs ? fit : regs;
+}
+
 // STATE: the segment's own state only (no output), for the sequences that are split into segments.
 template <typename T, int DA, int DC, bool VEC, bool STATE>
-__global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
+__global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC>())) void k_decay_chunk(DecayPass p, int ndc) {
     typedef Mm<T> M;
     typedef typename M::frag frag;
     typedef Lds<T, DA, DC> L;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
     constexpr int NB = C * DA / V / 256, NV = C * DC / V / 256;      // 16-byte pieces per thread of a chunk of b and c
     static_assert(NB >= 1 && NV >= 1, "a chunk is at least one piece per thread");
     extern __shared__ __align__(16) char lds[];
-    float *const pw = reinterpret_cast<float *>(lds + L::PW);
+    float *const pw = reinterpret_cast<float *>(lds + L::PW), *const uw = reinterpret_cast<float *>(lds + L::UW);
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
     // blocks of one XCD (block index mod 8) take neighbouring work: the heads of a token share cache lines, shared heads and column tiles share rows
@@ -184,7 +184,12 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
     const int64_t ot = (int64_t)p.H * p.dc;          // output elements per token
     const int64_t ob = ((int64_t)n * p.T * p.H + h) * p.dc + c0;
 
+    // pw[m] = e^{g m}; uw[x] = the state update's weight of a row that is followed by 63 - x others (0: there is no such row)
     if (tid <= C) pw[tid] = tid == 0 ? 1.f : expf(p.log_decay[h] * (float)tid);
+    if (tid < 2 * C) {
+        const int m = C - tid - o;
+        uw[tid] = tid >= C ? 0.f : m == 0 ? p.f_upd : p.f_upd * expf(p.log_decay[h] * (float)m);
+    }
 
     // ---- the state: rows a = 16 (a-tile) + 4 g + i, column c = 16 (c-tile) + l
     const int a_t0 = DA >= 64 ? w * NA : w & 1, c_t0 = DA >= 64 ? 0 : (w >> 1) * NCW;
@@ -205,45 +210,51 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
             }
         }
 
+    // rows of the next chunk: this thread's piece of b and c (16-byte pieces RPB, RPC rows apart) and its token's a row. Row pointers step by a whole chunk
+    constexpr int RPB = 256 / (DA / V), RPC = 256 / (DC / V);
     uint4 rb[NB], rc[NV];
     frag fa[KA], fa_next[KA];
+    const int dir = p.rev ? -1 : 1, first = p.rev ? len - 1 - u_lo : u_lo;
+    const int br = tid / (DA / V), bcol = tid % (DA / V) * V, cr = tid / (DC / V), ccol = tid % (DC / V) * V, ar = 16 * w + l;
+    const T *bq = bp + (int64_t)(first + dir * br) * p.bs[1] + bcol, *cq = cp + (int64_t)(first + dir * cr) * p.cs[1] + ccol;
+    const T *aq = ap + (int64_t)(first + dir * ar) * p.as[1] + g * V;
+    const int64_t bstep = dir * RPB * p.bs[1], cstep = dir * RPC * p.cs[1], astep = dir * C * p.as[1];
     auto fetch = [&](int u0) {
+        const int left = u_end - u0;                 // rows of the chunk that are there
 #pragma unroll
-        for (int x = 0; x < NB; ++x) {
-            const int v = x * 256 + tid, r = v / (DA / V), col = v % (DA / V) * V, u = u0 + r;
+        for (int x = 0; x < NB; ++x, bq += bstep) {
             rb[x] = make_uint4(0, 0, 0, 0);
-            if (u < u_end) rb[x] = load16<T, VEC>(bp + (int64_t)(p.rev ? len - 1 - u : u) * p.bs[1], col, p.da);
+            if (br + x * RPB < left) rb[x] = load16<T, VEC>(bq, p.da - bcol);
         }
 #pragma unroll
-        for (int x = 0; x < NV; ++x) {
-            const int v = x * 256 + tid, r = v / (DC / V), col = v % (DC / V) * V, u = u0 + r;
+        for (int x = 0; x < NV; ++x, cq += cstep) {
             rc[x] = make_uint4(0, 0, 0, 0);
-            if (u < u_end) rc[x] = load16<T, VEC>(cp + (int64_t)(p.rev ? len - 1 - u : u) * p.cs[1], col, dcw);
+            if (cr + x * RPC < left) rc[x] = load16<T, VEC>(cq, dcw - ccol);
         }
         if (!STATE) {
-            const int u = u0 + 16 * w + l;
-            const T *row = ap + (int64_t)(p.rev ? len - 1 - u : u) * p.as[1];
 #pragma unroll
             for (int k = 0; k < KA; ++k) {
                 union { uint4 u4; frag f; } t;
                 t.u4 = make_uint4(0, 0, 0, 0);
-                if (u < u_end) t.u4 = load16<T, VEC>(row, k * M::KB + g * V, p.da);
+                if (ar < left) t.u4 = load16<T, VEC>(aq + k * M::KB, p.da - k * M::KB - g * V);
                 fa_next[k] = t.f;
             }
+            aq += astep;
         }
     };
+    int64_t oi = ob + (int64_t)(first + dir * ar) * ot;
+    const int64_t ostep = dir * C * ot;
     if (u_lo < u_end) fetch(u_lo);
     __syncthreads();
 
-    // ---- weights that are the same in every chunk: pairs of token i = 16 w + l with j = 16 st + 4 g + e, and the update of a full chunk
-    float wp[4][4], wu[4][4];
+    // ---- weights of the pairs of token i = 16 w + l with j = 16 st + 4 g + e, the same in every chunk
+    float wp[4][4];
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int j = 16 * st + 4 * g + e, d = 16 * w + l - j;
             wp[st][e] = d >= 0 ? p.f_intra * pw[max(d, 0)] : 0.f;
-            wu[st][e] = p.f_upd * pw[C - j - o];
         }
     const float w_out = p.f_out * pw[16 * w + l + o];
 
@@ -251,15 +262,11 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
         const int cnt = min(C, u_end - u0);
         if (u0 > u_lo) __syncthreads();              // the products of the chunk before have read their tiles
 #pragma unroll
-        for (int x = 0; x < NB; ++x) {
-            const int v = x * 256 + tid;
-            *reinterpret_cast<uint4 *>(lds + L::B + v / (DA / V) * L::RB + v % (DA / V) * 16) = rb[x];
-        }
+        for (int x = 0; x < NB; ++x)
+            *reinterpret_cast<uint4 *>(lds + L::B + (br + x * RPB) * L::RB + bcol * (int)sizeof(T)) = rb[x];
 #pragma unroll
-        for (int x = 0; x < NV; ++x) {
-            const int v = x * 256 + tid;
-            *reinterpret_cast<uint4 *>(lds + L::C + v / (DC / V) * L::RC + v % (DC / V) * 16) = rc[x];
-        }
+        for (int x = 0; x < NV; ++x)
+            *reinterpret_cast<uint4 *>(lds + L::C + (cr + x * RPC) * L::RC + ccol * (int)sizeof(T)) = rc[x];
         if (!STATE) {
 #pragma unroll
             for (int x = 0; x < NA; ++x)
@@ -294,8 +301,7 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
                 M::split(acc, P[ks]);
             }
             // ---- out^T = w_out S^T a^T + c^T P^T
-            const int u = u0 + 16 * w + l;
-            const int64_t oi = ob + (int64_t)(p.rev ? len - 1 - u : u) * ot;
+            const bool there = u0 + ar < u_end;
 #pragma unroll
             for (int y = 0; y < NC; ++y) {
                 f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
                     for (int x = 0; x < M::NP; ++x) acc = M::mma(fc, P[ks][x], acc);
                 }
                 const int c = 16 * y + 4 * g;
-                if (u < u_end && c < dcw) {
+                if (there && c < dcw) {
                     if (p.out_f32) {
                         float *d = static_cast<float *>(p.out) + oi + c;
                         if (VEC) *reinterpret_cast<f32x4 *>(d) = acc;
@@ -342,12 +348,9 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
             }
         }
 
+        oi += ostep;
+
         // ---- S = e^{g cnt} S + (w b)^T c
-        if (cnt < C)
-#pragma unroll
-            for (int st = 0; st < 4; ++st)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wu[st][e] = p.f_upd * pw[max(cnt - (16 * st + 4 * g + e) - o, 0)];      // (rows behind cnt are zero)
         const float keep = pw[cnt];
 #pragma unroll
         for (int x = 0; x < NA; ++x)
@@ -357,10 +360,12 @@ __global__ __launch_bounds__(256, 1) void k_decay_chunk(DecayPass p, int ndc) {
                 for (int e = 0; e < 4; ++e) S[x][y][e] *= keep;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
+            float wu[M::TILES * 4];
+#pragma unroll
+            for (int e = 0; e < M::TILES * 4; ++e) wu[e] = uw[C - cnt + 16 * (ks * M::TILES + e / 4) + 4 * g + e % 4];
             frag fb[NA][M::NU];
 #pragma unroll
-            for (int x = 0; x < NA; ++x)
-                M::weigh(M::load_col(lds + L::B, L::RB, ks, g, 16 * (a_t0 + x) + l), &wu[ks * M::TILES][0], fb[x]);
+            for (int x = 0; x < NA; ++x) M::weigh(M::load_col(lds + L::B, L::RB, ks, g, 16 * (a_t0 + x) + l), wu, fb[x]);
 #pragma unroll
             for (int y = 0; y < NCW; ++y) {
                 const frag fc = M::load_col(lds + L::C, L::RC, ks, g, 16 * (c_t0 + y) + l);
