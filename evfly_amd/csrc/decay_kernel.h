@@ -137,18 +137,19 @@ template <typename T, int DA, int DC> struct Lds {
     static constexpr int RS = DA * (int)sizeof(T) + 16;
     static constexpr int PW = 0, UW = 272, B = 1024, C = B + DECAY_CHUNK * RB, S = C + DECAY_CHUNK * RC;
     static constexpr int PLANE = DC * RS;
-    static constexpr int BYTES = S + PLANE * Mm<T>::NP;
+    static constexpr int STATE_BYTES = S, BYTES = S + PLANE * Mm<T>::NP;      // (a pass for the state alone has no use for S as an operand)
 };
 
 // Blocks that share a CU: as many as LDS and registers hold without spills.
-template <typename T, int DA, int DC> constexpr int blocks_per_cu() {
-    constexpr int regs = sizeof(T) == 4 ? (DA == 128 ? 2 : DA == 64 ? 3 : 4) : DA == 128 ? 3 : 4, fit = kMaxLds / Lds<T, DA, DC>::BYTES;
+template <typename T, int DA, int DC, bool STATE> constexpr int blocks_per_cu() {
+    constexpr int regs = sizeof(T) == 4 ? (DA == 128 ? 2 : DA == 64 ? 3 : 4) : DA == 128 ? 3 : 4;
+    constexpr int fit = kMaxLds / (STATE ? Lds<T, DA, DC>::STATE_BYTES : Lds<T, DA, DC>::BYTES);
     return fit < regs ? fit : regs;
 }
 
 // STATE: the segment's own state only (no output), for the sequences that are split into segments.
 template <typename T, int DA, int DC, bool VEC, bool STATE>
-__global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC>())) void k_decay_chunk(DecayPass p, int ndc) {
+__global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_decay_chunk(DecayPass p, int ndc) {
     typedef Mm<T> M;
     typedef typename M::frag frag;
     typedef Lds<T, DA, DC> L;
@@ -158,12 +159,16 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC>())) void k_decay_chu
     constexpr int NC = DC / 16;                      // 16-column tiles of c
     constexpr int NA = DA >= 64 ? DA / 64 : 1;       // the wave's share of the state: NA a-tiles by NCW c-tiles
     constexpr int NCW = DA >= 64 ? NC : NC / 2;
+    // pairs whose weights are all zero (later tokens): fp32, bound by its products, leaves them out; in bf16 the branches around them cost more
+    constexpr bool SKIP = sizeof(T) == 4;
     constexpr int NB = C * DA / V / 256, NV = C * DC / V / 256;      // 16-byte pieces per thread of a chunk of b and c
     static_assert(NB >= 1 && NV >= 1, "a chunk is at least one piece per thread");
     extern __shared__ __align__(16) char lds[];
     float *const pw = reinterpret_cast<float *>(lds + L::PW), *const uw = reinterpret_cast<float *>(lds + L::UW);
 
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
+    // (every other block hands its tokens to the waves in the opposite order: later tokens have more pairs)
+    const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wt = SKIP && (blockIdx.x / kNumXCD & 1) ? 3 - w : w;
     // blocks of one XCD (block index mod 8) take neighbouring work: the heads of a token share cache lines, shared heads and column tiles share rows
     const int total = gridDim.x, q8 = total / kNumXCD, r8 = total % kNumXCD, xcd = blockIdx.x % kNumXCD;
     int id = xcd * q8 + min(xcd, r8) + blockIdx.x / kNumXCD;
@@ -215,7 +220,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC>())) void k_decay_chu
     uint4 rb[NB], rc[NV];
     frag fa[KA], fa_next[KA];
     const int dir = p.rev ? -1 : 1, first = p.rev ? len - 1 - u_lo : u_lo;
-    const int br = tid / (DA / V), bcol = tid % (DA / V) * V, cr = tid / (DC / V), ccol = tid % (DC / V) * V, ar = 16 * w + l;
+    const int br = tid / (DA / V), bcol = tid % (DA / V) * V, cr = tid / (DC / V), ccol = tid % (DC / V) * V, ar = 16 * wt + l;
     const T *bq = bp + (int64_t)(first + dir * br) * p.bs[1] + bcol, *cq = cp + (int64_t)(first + dir * cr) * p.cs[1] + ccol;
     const T *aq = ap + (int64_t)(first + dir * ar) * p.as[1] + g * V;
     const int64_t bstep = dir * RPB * p.bs[1], cstep = dir * RPC * p.cs[1], astep = dir * C * p.as[1];
@@ -247,16 +252,16 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC>())) void k_decay_chu
     if (u_lo < u_end) fetch(u_lo);
     __syncthreads();
 
-    // ---- weights of the pairs of token i = 16 w + l with j = 16 st + 4 g + e, the same in every chunk
+    // ---- weights of the pairs of token i = 16 wt + l with j = 16 st + 4 g + e, the same in every chunk
     float wp[4][4];
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int j = 16 * st + 4 * g + e, d = 16 * w + l - j;
+            const int j = 16 * st + 4 * g + e, d = 16 * wt + l - j;
             wp[st][e] = d >= 0 ? p.f_intra * pw[max(d, 0)] : 0.f;
         }
-    const float w_out = p.f_out * pw[16 * w + l + o];
+    const float w_out = p.f_out * pw[16 * wt + l + o];
 
     for (int u0 = u_lo; u0 < u_end; u0 += C) {
         const int cnt = min(C, u_end - u0);
@@ -284,19 +289,18 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC>())) void k_decay_chu
             frag P[KS][M::NP];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                if (ks * M::TILES > w) continue;
+                if (SKIP && ks * M::TILES > wt) continue;
                 f32x4 acc[M::TILES];
 #pragma unroll
                 for (int x = 0; x < M::TILES; ++x) {
                     const int st = ks * M::TILES + x;
                     acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (st > w) continue;
+                    if (SKIP && st > wt) continue;
 #pragma unroll
                     for (int k = 0; k < KA; ++k)
                         acc[x] = M::mma(M::load(lds + L::B + (16 * st + l) * L::RB + k * 64 + g * 16), fa[k], acc[x]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)          // a later token's product is dropped, not multiplied by zero
-                        acc[x][e] = st < w || 4 * g + e <= l ? acc[x][e] * wp[st][e] : 0.f;
+                    for (int e = 0; e < 4; ++e) acc[x][e] *= wp[st][e];
                 }
                 M::split(acc, P[ks]);
             }
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC>())) void k_decay_chu
                 for (int e = 0; e < 4; ++e) acc[e] *= w_out;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    if (ks * M::TILES > w) continue;
+                    if (SKIP && ks * M::TILES > wt) continue;
                     const frag fc = M::load_col(lds + L::C, L::RC, ks, g, 16 * y + l);
 #pragma unroll
                     for (int x = 0; x < M::NP; ++x) acc = M::mma(fc, P[ks][x], acc);
@@ -442,11 +446,11 @@ template <typename T, int DA, int DC, bool VEC> int launch(const DecayPass &p, c
     EVFLY_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
     if (!attr_set[dev].load(std::memory_order_acquire)) {
         EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_decay_chunk<T, DA, DC, VEC, false>), hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES));
-        EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_decay_chunk<T, DA, DC, VEC, true>), hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES));
+        EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_decay_chunk<T, DA, DC, VEC, true>), hipFuncAttributeMaxDynamicSharedMemorySize, L::STATE_BYTES));
         attr_set[dev].store(true, std::memory_order_release);
     }
     if (pl.nseg > 1) {
-        hipLaunchKernelGGL((k_decay_chunk<T, DA, DC, VEC, true>), dim3((unsigned)(tiles * (pl.nseg - 1))), dim3(256), L::BYTES, st, p, pl.ndc);
+        hipLaunchKernelGGL((k_decay_chunk<T, DA, DC, VEC, true>), dim3((unsigned)(tiles * (pl.nseg - 1))), dim3(256), L::STATE_BYTES, st, p, pl.ndc);
         hipLaunchKernelGGL((k_decay_scan<DA, DC>), dim3((unsigned)tiles, DA * DC / 1024), dim3(256), 0, st, p, pl.ndc);
     }
     hipLaunchKernelGGL((k_decay_chunk<T, DA, DC, VEC, false>), dim3((unsigned)(tiles * pl.nseg)), dim3(256), L::BYTES, st, p, pl.ndc);
