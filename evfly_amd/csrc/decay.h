@@ -22,20 +22,27 @@ struct DecayPass {
     const float *s_in;               // state the pass starts from (NULL: zeros)
     float *s_fin;                    // state behind the pass (NULL: not wanted); may be s_in
     int64_t s_a, s_c;                // element strides of the state's a and c dimension
-    float *seg;                      // states of the segments (nseg > 1)
+    float *seg;                      // states the segments start from, [stream, head][segment][dk][dv] (nseg > 1)
     int n, T, H, da, dc, nseg, seg_len;
     int rev;                         // token order: 0 first to last, 1 last to first
     float f_intra, f_out, f_upd;     // where the operator's scale enters: pair products, state read, state update
 };
 
-// Plan of a pass: tiles and the split of the sequence into segments that run side by side.
-struct DecayPlan {
-    int DA, DC, ndc, nseg, seg_len;
-    int64_t seg_floats;              // workspace of the segment states
+// Passes of one launch (the same tiles): neighbouring blocks run the passes of one place, so that rows that several of them read come from L2.
+struct DecayPasses {
+    DecayPass p[3];
+    int np;
 };
-DecayPlan decay_plan(int n, int T, int H, int da, int dc);
 
-int decay_pass_f32(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st);
-int decay_pass_bf16(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st);
+// Split of the sequence into segments that run side by side.
+struct DecaySplit { int nseg, seg_len; };
+DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype);
+
+// All passes have the same da and dc classes. STATE: the segments' own states only (into slot segment + 1 of seg), no output.
+int decay_passes_f32(const DecayPasses &p, bool state, bool vec, hipStream_t st);
+int decay_passes_bf16(const DecayPasses &p, bool state, bool vec, hipStream_t st);
+
+inline int decay_tile_a(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }      // the a dimension whole (its rows are summed in registers)
+inline int decay_tile_c(int d) { return d <= 32 ? 32 : 64; }                       // columns of c per block
 
 }  // namespace evfly

@@ -116,21 +116,59 @@ template <typename T> int step_all(const StepArgs &a, int n, hipStream_t st) {
     return a.dv <= 32 ? step_launch<T, 1, 32>(a, n, st) : a.dv <= 64 ? step_launch<T, 1, 64>(a, n, st) : step_launch<T, 1, 128>(a, n, st);
 }
 
+// ---------------------------------------------------------------------------------------- states at the segment borders
+// slot s + 1 holds segment s's own state (the tokens of that segment alone); slot s receives the state that segment s starts from,
+//     start_{s+1} = e^{g cnt_s} start_s + own_s,    start_0 = s_in
+// (start_0 as well: the last segment may write its final state over s_in while the first one runs). Segments count in the pass's own order of time.
+struct ScanArgs {
+    float *slots[2];
+    const float *s_in[2];
+    const float *log_decay;
+    const int32_t *lengths;
+    int T, H, nseg, seg_len, elems;       // elems = dk * dv
+};
+__global__ __launch_bounds__(256) void k_decay_scan(ScanArgs p) {
+    const int i = blockIdx.y * 256 + threadIdx.x, nh = blockIdx.x, z = blockIdx.z;
+    if (i >= p.elems) return;
+    const int len = p.lengths ? min(max(p.lengths[nh / p.H], 0), p.T) : p.T;
+    const float gl = p.log_decay[nh % p.H];
+    float *slot = p.slots[z] + (int64_t)nh * p.nseg * p.elems + i;
+    float S = p.s_in[z] ? p.s_in[z][(int64_t)nh * p.elems + i] : 0.f;
+    slot[0] = S;
+    const float full = expf(gl * (float)p.seg_len);
+#pragma unroll 8
+    for (int s = 1; s < p.nseg; ++s) {
+        const int cnt = min(max(len - (s - 1) * p.seg_len, 0), p.seg_len);
+        const float keep = cnt == p.seg_len ? full : cnt == 0 ? 1.f : expf(gl * (float)cnt);
+        S = fmaf(keep, S, slot[(int64_t)s * p.elems]);
+        slot[(int64_t)s * p.elems] = S;
+    }
+}
+
 // ---------------------------------------------------------------------------------------- sum over the heads that share a key / value head
-// in (rows, kv, rep, d) fp32 -> out (rows, kv, d), added in head order
-template <typename T> __global__ __launch_bounds__(256) void k_decay_head_sum(const float *in, int64_t n, int rep, int d, T *out) {
+// in (rows, kv, rep, d) fp32 -> out (rows, kv, d), added in head order; blockIdx.y: dk or dv
+struct HeadSum {
+    const float *in[2];
+    void *out[2];
+    int d[2];
+    int64_t heads;                         // rows * kv
+    int rep;
+};
+template <typename T> __global__ __launch_bounds__(256) void k_decay_head_sum(HeadSum p) {
+    const int y = blockIdx.y, d = p.d[y];
+    const int64_t n = p.heads * d;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / d;
-        const float *s = in + row * rep * d + i % d;
+        const int64_t head = i / d;
+        const float *s = p.in[y] + head * p.rep * d + (i - head * d);
         float a = 0.f;
-        for (int r = 0; r < rep; ++r) a += s[(int64_t)r * d];
-        Elem<T>::st1(out + i, a);
+        for (int r = 0; r < p.rep; ++r) a += s[(int64_t)r * d];
+        Elem<T>::st1(static_cast<T *>(p.out[y]) + i, a);
     }
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-struct Tokens {              // one token tensor: pointer, element strides, heads per head of the pass, width
+struct Tokens {              // one token tensor: pointer, element strides, heads of the pass per head of it, width
     const void *p;
     int64_t s[3];
     int r, d;
@@ -139,32 +177,49 @@ bool vec_ok(const Tokens &t, int vec) {
     return aligned16(t.p) && t.d % vec == 0 && t.s[0] % vec == 0 && t.s[1] % vec == 0 && t.s[2] % vec == 0;
 }
 
-int run_pass(DecayPass p, const Tokens &a, const Tokens &b, const Tokens &c, int dtype, float *seg, hipStream_t st) {
-    p.a = a.p; p.b = b.p; p.c = c.p;
-    for (int i = 0; i < 3; ++i) { p.as[i] = a.s[i]; p.bs[i] = b.s[i]; p.cs[i] = c.s[i]; }
-    p.ra = a.r; p.rb = b.r; p.rc = c.r;
-    p.da = a.d; p.dc = c.d;
-    const DecayPlan pl = decay_plan(p.n, p.T, p.H, p.da, p.dc);
-    p.nseg = pl.nseg; p.seg_len = pl.seg_len; p.seg = seg;
-    const int vec = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
-    const bool v = vec_ok(a, vec) && vec_ok(b, vec) && vec_ok(c, vec) && aligned16(p.out);
-    return dtype == EVFLY_DTYPE_F32 ? decay_pass_f32(p, pl, v, st) : decay_pass_bf16(p, pl, v, st);
-}
+// One call's passes: roles filled in, tiles chosen, launched together where the tiles agree.
+struct Run {
+    int dtype;
+    bool vec = true;                       // every tensor of the call in 16-byte pieces
+    hipStream_t st;
+    DecayPass base;                        // what all passes share
 
-struct Ws { int64_t seg, part, bytes; };      // offsets in bytes
-Ws decay_ws(int n, int T, int H, int KV, int dk, int dv, bool backward) {
-    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-    Ws w{0, 0, 0};
-    int64_t seg = 0;
-    if (T > EVFLY_DECAY_STEP_TOKENS || backward) {
-        seg = decay_plan(n, T, H, dk, dv).seg_floats;
-        if (backward) {
-            const int64_t t = decay_plan(n, T, H, dv, dk).seg_floats;
-            seg = seg > t ? seg : t;
-        }
+    DecayPass pass(const Tokens &a, const Tokens &b, const Tokens &c) const {
+        DecayPass p = base;
+        p.a = a.p; p.b = b.p; p.c = c.p;
+        for (int i = 0; i < 3; ++i) { p.as[i] = a.s[i]; p.bs[i] = b.s[i]; p.cs[i] = c.s[i]; }
+        p.ra = a.r; p.rb = b.r; p.rc = c.r;
+        p.da = a.d; p.dc = c.d;
+        return p;
     }
-    w.part = up(seg * 4);
-    w.bytes = w.part + (backward && H != KV ? up((int64_t)n * T * H * (dk > dv ? dk : dv) * 4) : 0);
+    int launch(const DecayPasses &ps, bool state) const {
+        return dtype == EVFLY_DTYPE_F32 ? decay_passes_f32(ps, state, vec, st) : decay_passes_bf16(ps, state, vec, st);
+    }
+    // slots of up to two state sequences [dk][dv], each from its own state pass
+    int segment_states(const DecayPass *own, int np, int dk, int dv) const {
+        DecayPasses ps{};
+        ScanArgs sc{};
+        ps.np = np;
+        for (int i = 0; i < np; ++i) { ps.p[i] = own[i]; sc.slots[i] = own[i].seg; sc.s_in[i] = own[i].s_in; }
+        if (int rc = launch(ps, true)) return rc;
+        sc.log_decay = base.log_decay; sc.lengths = base.lengths; sc.T = base.T; sc.H = base.H; sc.nseg = base.nseg; sc.seg_len = base.seg_len; sc.elems = dk * dv;
+        hipLaunchKernelGGL(k_decay_scan, dim3((unsigned)(base.n * base.H), (dk * dv + 255) / 256, np), dim3(256), 0, st, sc);
+        EVFLY_LAUNCH_CHECK();
+        return 0;
+    }
+};
+
+struct Ws { int64_t seg_floats, part_k, part_v, bytes; };      // part_*: offsets in bytes
+Ws decay_ws(int n, int T, int H, int KV, int dk, int dv, int dtype, bool backward) {
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    Ws w{0, 0, 0, 0};
+    if (T > EVFLY_DECAY_STEP_TOKENS || backward) {
+        const DecaySplit sp = decay_split(n, T, H, dk, dv, dtype);
+        if (sp.nseg > 1) w.seg_floats = up((int64_t)n * H * sp.nseg * dk * dv * 4) / 4;
+    }
+    w.part_k = w.seg_floats * 4 * (backward ? 2 : 1);
+    w.part_v = w.part_k + (backward && H != KV ? up((int64_t)n * T * H * dk * 4) : 0);
+    w.bytes = w.part_v + (backward && H != KV ? up((int64_t)n * T * H * dv * 4) : 0);
     return w;
 }
 
@@ -185,14 +240,10 @@ void token_strides(const int64_t *s, int T, int heads, int d, int64_t (&out)[3])
 
 }  // namespace
 
-// Tiles: the a dimension whole (its rows are summed in registers), 64 columns of c per block (32 if there are no more). Segments: the sequence is cut where there are
-// fewer than four blocks per CU, into pieces of at least four chunks -- a cut costs the rows b and c a second read and the state a round trip.
-DecayPlan decay_plan(int n, int T, int H, int da, int dc) {
-    DecayPlan p;
-    p.DA = da <= 32 ? 32 : da <= 64 ? 64 : 128;
-    p.DC = dc <= 32 ? 32 : 64;
-    p.ndc = (dc + p.DC - 1) / p.DC;
-    const int64_t base = (int64_t)n * H * p.ndc;
+// The sequence is cut where there are fewer than four blocks per CU, into pieces of at least four chunks: a cut costs two of the four token tensors a
+// second read and the state a round trip.
+DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype) {
+    const int64_t base = (int64_t)n * H * ((dv + decay_tile_c(dv) - 1) / decay_tile_c(dv));
     int64_t nseg = base > 0 ? (4 * kNumCU + base - 1) / base : 1;
     const int64_t most = (T + 4 * DECAY_CHUNK - 1) / (4 * DECAY_CHUNK);
     nseg = nseg < most ? nseg : most;
@@ -200,11 +251,8 @@ DecayPlan decay_plan(int n, int T, int H, int da, int dc) {
     int64_t len = (T + nseg - 1) / nseg;
     len = (len + DECAY_CHUNK - 1) / DECAY_CHUNK * DECAY_CHUNK;
     if (len < DECAY_CHUNK) len = DECAY_CHUNK;
-    p.seg_len = (int)len;
-    p.nseg = (int)((T + len - 1) / len);
-    if (p.nseg < 1) p.nseg = 1;
-    p.seg_floats = p.nseg > 1 ? base * p.nseg * p.DA * p.DC : 0;
-    return p;
+    nseg = (T + len - 1) / len;
+    return DecaySplit{(int)(nseg > 1 ? nseg : 1), (int)len};
 }
 
 }  // namespace evfly
@@ -214,7 +262,7 @@ using namespace evfly;
 extern "C" int64_t evfly_decay_attention_workspace_bytes(int n_streams, int tokens, int heads, int kv_heads, int dk, int dv, int dtype,
                                                          int backward) {
     if (check_shape("decay_attention_workspace_bytes", n_streams, tokens, heads, kv_heads, dk, dv, dtype, 1.f)) return -1;
-    return decay_ws(n_streams, tokens, heads, kv_heads, dk, dv, backward != 0).bytes;
+    return decay_ws(n_streams, tokens, heads, kv_heads, dk, dv, dtype, backward != 0).bytes;
 }
 
 extern "C" int evfly_decay_attention_forward(const void *q, const void *k, const void *v, const int64_t *strides_host,
@@ -224,7 +272,7 @@ extern "C" int evfly_decay_attention_forward(const void *q, const void *k, const
     if (int rc = check_shape("decay_attention_forward", n_streams, tokens, heads, kv_heads, dk, dv, dtype, scale)) return rc;
     if (n_streams == 0) return 0;
     EVFLY_REQUIRE(log_decay && (tokens == 0 || (q && k && v && out)), "decay_attention_forward: null argument");
-    const Ws ws = decay_ws(n_streams, tokens, heads, kv_heads, dk, dv, false);
+    const Ws ws = decay_ws(n_streams, tokens, heads, kv_heads, dk, dv, dtype, false);
     EVFLY_REQUIRE(workspace_bytes >= ws.bytes && (ws.bytes == 0 || (workspace && aligned16(workspace))),
                   "decay_attention_forward: workspace smaller than evfly_decay_attention_workspace_bytes, or not 16-byte aligned");
     hipStream_t st = as_stream(stream);
@@ -241,11 +289,19 @@ extern "C" int evfly_decay_attention_forward(const void *q, const void *k, const
         a.T = tokens; a.H = heads; a.rep = rep; a.dk = dk; a.dv = dv; a.scale = scale;
         return dtype == EVFLY_DTYPE_F32 ? step_all<float>(a, n_streams, st) : step_all<bf16_t>(a, n_streams, st);
     }
-    DecayPass p{};
-    p.out = out; p.log_decay = log_decay; p.lengths = lengths; p.n = n_streams; p.T = tokens; p.H = heads;
-    p.s_in = state_in; p.s_fin = state_out; p.s_a = dv; p.s_c = 1;
-    p.f_intra = scale; p.f_out = scale; p.f_upd = 1.f;
-    return run_pass(p, tq, tk, tv, dtype, static_cast<float *>(workspace), st);
+    const int vec = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
+    Run run{dtype, vec_ok(tq, vec) && vec_ok(tk, vec) && vec_ok(tv, vec) && aligned16(out), st, DecayPass{}};
+    const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype);
+    DecayPass &b = run.base;
+    b.log_decay = log_decay; b.lengths = lengths; b.n = n_streams; b.T = tokens; b.H = heads; b.nseg = sp.nseg; b.seg_len = sp.seg_len;
+    b.seg = static_cast<float *>(workspace); b.s_in = state_in; b.s_a = dv; b.s_c = 1;
+    DecayPasses ps{};
+    ps.np = 1;
+    ps.p[0] = run.pass(tq, tk, tv);
+    ps.p[0].out = out; ps.p[0].s_fin = state_out; ps.p[0].f_intra = scale; ps.p[0].f_out = scale; ps.p[0].f_upd = 1.f;
+    if (sp.nseg > 1)
+        if (int rc = run.segment_states(ps.p, 1, dk, dv)) return rc;
+    return run.launch(ps, false);
 }
 
 extern "C" int evfly_decay_attention_backward(const void *q, const void *k, const void *v, const int64_t *strides_host,
@@ -256,7 +312,7 @@ extern "C" int evfly_decay_attention_backward(const void *q, const void *k, cons
     if (int rc = check_shape("decay_attention_backward", n_streams, tokens, heads, kv_heads, dk, dv, dtype, scale)) return rc;
     if (n_streams == 0) return 0;
     EVFLY_REQUIRE(log_decay && (tokens == 0 || (q && k && v && d_out && dq && dk_out && dv_out)), "decay_attention_backward: null argument");
-    const Ws ws = decay_ws(n_streams, tokens, heads, kv_heads, dk, dv, true);
+    const Ws ws = decay_ws(n_streams, tokens, heads, kv_heads, dk, dv, dtype, true);
     EVFLY_REQUIRE(workspace_bytes >= ws.bytes && (ws.bytes == 0 || (workspace && aligned16(workspace))),
                   "decay_attention_backward: workspace smaller than evfly_decay_attention_workspace_bytes, or not 16-byte aligned");
     hipStream_t st = as_stream(stream);
@@ -266,37 +322,52 @@ extern "C" int evfly_decay_attention_backward(const void *q, const void *k, cons
     token_strides(strides_host ? strides_host + 3 : nullptr, tokens, kv_heads, dk, tk.s);
     token_strides(strides_host ? strides_host + 6 : nullptr, tokens, kv_heads, dv, tv.s);
     token_strides(nullptr, tokens, heads, dv, to.s);
+    EVFLY_REQUIRE(!d_state_in || d_state_in != d_state_out, "decay_attention_backward: d_state_in is d_state_out");
+    const int vec = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
+    Run run{dtype, vec_ok(tq, vec) && vec_ok(tk, vec) && vec_ok(tv, vec) && vec_ok(to, vec) && aligned16(dq) && aligned16(dk_out) && aligned16(dv_out), st, DecayPass{}};
+    const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype);
     char *const w = static_cast<char *>(workspace);
-    float *const seg = reinterpret_cast<float *>(w), *const part = reinterpret_cast<float *>(w + ws.part);
+    float *const seg = reinterpret_cast<float *>(w), *const part_k = reinterpret_cast<float *>(w + ws.part_k), *const part_v = reinterpret_cast<float *>(w + ws.part_v);
+    DecayPass &b = run.base;
+    b.log_decay = log_decay; b.lengths = lengths; b.n = n_streams; b.T = tokens; b.H = heads; b.nseg = sp.nseg; b.seg_len = sp.seg_len;
+    b.f_intra = scale;
 
-    DecayPass p{};
-    p.log_decay = log_decay; p.lengths = lengths; p.n = n_streams; p.T = tokens; p.H = heads;
-    // dq_t = scale sum_{s <= t} e^{g (t - s)} (d_out_t . v_s) k_s + scale e^{g (t + 1)} S_in d_out_t
-    DecayPass a = p;
-    a.out = dq; a.s_in = state_in; a.s_a = 1; a.s_c = dv; a.f_intra = scale; a.f_out = scale; a.f_upd = 1.f;
-    if (tokens > 0)
-        if (int rc = run_pass(a, to, tv, tk, dtype, seg, st)) return rc;
-    // dk_s = scale sum_{t >= s} e^{g (t - s)} (v_s . d_out_t) q_t + e^{g (T - 1 - s)} d_state_out v_s
-    DecayPass b = p;
-    b.rev = 1; b.out = rep > 1 ? static_cast<void *>(part) : dk_out; b.out_f32 = rep > 1;
-    b.s_in = d_state_out; b.s_a = 1; b.s_c = dv; b.f_intra = scale; b.f_out = 1.f; b.f_upd = scale;
-    auto head_sum = [&](void *out, int d) {
-        const int64_t rows = (int64_t)n_streams * tokens * kv_heads, m = rows * d;
-        const unsigned blocks = (unsigned)(m / 256 + 1 < 8 * kNumCU ? m / 256 + 1 : 8 * kNumCU);
-        if (dtype == EVFLY_DTYPE_F32) hipLaunchKernelGGL(k_decay_head_sum<float>, dim3(blocks), dim3(256), 0, st, part, m, rep, d, static_cast<float *>(out));
-        else hipLaunchKernelGGL(k_decay_head_sum<bf16_t>, dim3(blocks), dim3(256), 0, st, part, m, rep, d, static_cast<bf16_t *>(out));
-    };
-    if (tokens > 0) {
-        if (int rc = run_pass(b, tv, to, tq, dtype, seg, st)) return rc;
-        if (rep > 1) head_sum(dk_out, dk);
+    // dq_t = scale sum_{s <= t} e^{g (t - s)} (d_out_t . v_s) k_s + scale e^{g (t + 1)} S_in d_out_t: the state's own sequence, read transposed
+    DecayPass pq = run.pass(to, tv, tk);
+    pq.out = dq; pq.seg = seg; pq.s_in = state_in; pq.s_a = 1; pq.s_c = dv; pq.f_out = scale; pq.f_upd = 1.f;
+    // dk_s = scale sum_{t >= s} e^{g (t - s)} (v_s . d_out_t) q_t + e^{g (T - 1 - s)} d_state_out v_s: backwards over the state's gradient, read transposed
+    DecayPass pk = run.pass(tv, to, tq);
+    pk.rev = 1; pk.out = rep > 1 ? static_cast<void *>(part_k) : dk_out; pk.out_f32 = rep > 1;
+    pk.seg = seg + ws.seg_floats; pk.s_in = d_state_out; pk.s_a = 1; pk.s_c = dv; pk.f_out = 1.f; pk.f_upd = scale;
+    // dv_s = scale sum_{t >= s} e^{g (t - s)} (k_s . q_t) d_out_t + e^{g (T - 1 - s)} d_state_out^T k_s; the state it ends with is state_in's gradient
+    DecayPass pv = run.pass(tk, tq, to);
+    pv.rev = 1; pv.out = rep > 1 ? static_cast<void *>(part_v) : dv_out; pv.out_f32 = rep > 1;
+    pv.seg = seg + ws.seg_floats; pv.s_in = d_state_out; pv.s_fin = d_state_in; pv.s_a = dv; pv.s_c = 1; pv.f_out = 1.f; pv.f_upd = scale;
+    if (sp.nseg > 1) {
+        // the state k v^T and its gradient q d_out^T, both [dk][dv]
+        DecayPass own[2] = {run.pass(tk, tk, tv), pv};
+        own[0].seg = seg; own[0].s_in = state_in; own[0].s_a = dv; own[0].s_c = 1; own[0].f_upd = 1.f;
+        if (int rc = run.segment_states(own, 2, dk, dv)) return rc;
     }
-    // dv_s = scale sum_{t >= s} e^{g (t - s)} (k_s . q_t) d_out_t + e^{g (T - 1 - s)} d_state_out^T k_s; the state that this pass ends with is the
-    // gradient of state_in
-    DecayPass c = p;
-    c.rev = 1; c.out = rep > 1 ? static_cast<void *>(part) : dv_out; c.out_f32 = rep > 1;
-    c.s_in = d_state_out; c.s_fin = d_state_in; c.s_a = dv; c.s_c = 1; c.f_intra = scale; c.f_out = 1.f; c.f_upd = scale;
-    if (int rc = run_pass(c, tk, tq, to, dtype, seg, st)) return rc;
-    if (rep > 1 && tokens > 0) head_sum(dv_out, dv);
+    DecayPasses ps{};
+    ps.p[0] = pq; ps.p[1] = pk; ps.p[2] = pv;
+    if (decay_tile_a(dk) == decay_tile_a(dv) && decay_tile_c(dk) == decay_tile_c(dv) && (dk + decay_tile_c(dk) - 1) / decay_tile_c(dk) == (dv + decay_tile_c(dv) - 1) / decay_tile_c(dv)) {
+        ps.np = 3;
+        if (int rc = run.launch(ps, false)) return rc;
+    } else {
+        ps.np = 2;
+        if (int rc = run.launch(ps, false)) return rc;
+        ps.np = 1;
+        ps.p[0] = pv;
+        if (int rc = run.launch(ps, false)) return rc;
+    }
+    if (rep > 1 && tokens > 0) {
+        HeadSum h{{part_k, part_v}, {dk_out, dv_out}, {dk, dv}, (int64_t)n_streams * tokens * kv_heads, rep};
+        const int64_t need = (h.heads * (dk > dv ? dk : dv) + 255) / 256;
+        const dim3 grid((unsigned)(need < 8 * kNumCU ? need : 8 * kNumCU), 2);
+        if (dtype == EVFLY_DTYPE_F32) hipLaunchKernelGGL(k_decay_head_sum<float>, grid, dim3(256), 0, st, h);
+        else hipLaunchKernelGGL(k_decay_head_sum<bf16_t>, grid, dim3(256), 0, st, h);
+    }
     EVFLY_LAUNCH_CHECK();
     return 0;
 }

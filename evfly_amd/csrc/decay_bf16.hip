@@ -4,5 +4,5 @@
 #include "decay_kernel.h"
 
 namespace evfly {
-int decay_pass_bf16(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st) { return decay::launch_all<bf16_t>(p, pl, vec, st); }
+int decay_passes_bf16(const DecayPasses &p, bool state, bool vec, hipStream_t st) { return decay::launch_all<bf16_t>(p, state, vec, st); }
 }  // namespace evfly

@@ -142,14 +142,14 @@ template <typename T, int DA, int DC> struct Lds {
 
 // Blocks that share a CU: as many as LDS and registers hold without spills.
 template <typename T, int DA, int DC, bool STATE> constexpr int blocks_per_cu() {
-    constexpr int regs = sizeof(T) == 4 ? (DA == 128 ? 2 : DA == 64 ? 3 : 4) : DA == 128 ? 3 : 4;
+    constexpr int regs = DA == 128 ? (sizeof(T) == 4 ? 2 : 3) : sizeof(T) == 4 ? 3 : 4;
     constexpr int fit = kMaxLds / (STATE ? Lds<T, DA, DC>::STATE_BYTES : Lds<T, DA, DC>::BYTES);
     return fit < regs ? fit : regs;
 }
 
 // STATE: the segment's own state only (no output), for the sequences that are split into segments.
 template <typename T, int DA, int DC, bool VEC, bool STATE>
-__global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_decay_chunk(DecayPass p, int ndc) {
+__global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_decay_chunk(DecayPasses ps) {
     typedef Mm<T> M;
     typedef typename M::frag frag;
     typedef Lds<T, DA, DC> L;
@@ -172,7 +172,8 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
     // blocks of one XCD (block index mod 8) take neighbouring work: the heads of a token share cache lines, shared heads and column tiles share rows
     const int total = gridDim.x, q8 = total / kNumXCD, r8 = total % kNumXCD, xcd = blockIdx.x % kNumXCD;
     int id = xcd * q8 + min(xcd, r8) + blockIdx.x / kNumXCD;
-    const int nseg = STATE ? p.nseg - 1 : p.nseg;
+    const DecayPass &p = ps.p[id % ps.np]; id /= ps.np;
+    const int nseg = STATE ? p.nseg - 1 : p.nseg, ndc = (p.dc + DC - 1) / DC;
     const int c0 = (id % ndc) * DC; id /= ndc;
     const int h = id % p.H; id /= p.H;
     const int seg = id % nseg;
@@ -199,21 +200,21 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
     // ---- the state: rows a = 16 (a-tile) + 4 g + i, column c = 16 (c-tile) + l
     const int a_t0 = DA >= 64 ? w * NA : w & 1, c_t0 = DA >= 64 ? 0 : (w >> 1) * NCW;
     f32x4 S[NA][NCW];
-    const int tile_id = ((n * p.H + h) * ndc + c0 / DC);
-    float *const slots = p.seg + (int64_t)tile_id * p.nseg * (DA * DC);      // (nseg > 1)
+    float *const slots = p.seg + st_base * p.nseg;                           // (nseg > 1)
+    const int64_t state_n = (int64_t)p.da * p.dc;
+    const float *const start = STATE ? nullptr : p.nseg > 1 ? slots + seg * state_n : p.s_in ? p.s_in + st_base : nullptr;
+    auto each_state = [&](auto fn) {
 #pragma unroll
-    for (int x = 0; x < NA; ++x)
+        for (int x = 0; x < NA; ++x)
 #pragma unroll
-        for (int y = 0; y < NCW; ++y) {
-            if (!STATE && p.nseg > 1) {
-                S[x][y] = *reinterpret_cast<const f32x4 *>(slots + (int64_t)seg * (DA * DC) + ((x * NCW + y) * 256 + tid) * 4);
-            } else {
-                const int a = 16 * (a_t0 + x) + 4 * g, c = 16 * (c_t0 + y) + l;
+            for (int y = 0; y < NCW; ++y)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    S[x][y][i] = !STATE && p.s_in && a + i < p.da && c < dcw ? p.s_in[st_base + (a + i) * p.s_a + (c0 + c) * p.s_c] : 0.f;
-            }
-        }
+                for (int i = 0; i < 4; ++i) {
+                    const int a = 16 * (a_t0 + x) + 4 * g + i, c = 16 * (c_t0 + y) + l;
+                    S[x][y][i] = fn(S[x][y][i], a < p.da && c < dcw, a * p.s_a + (c0 + c) * p.s_c);
+                }
+    };
+    each_state([&](float, bool in, int64_t at) { return start && in ? start[at] : 0.f; });
 
     // rows of the next chunk: this thread's piece of b and c (16-byte pieces RPB, RPC rows apart) and its token's a row. Row pointers step by a whole chunk
     constexpr int RPB = 256 / (DA / V), RPC = 256 / (DC / V);
@@ -382,11 +383,8 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
     }
 
     if (STATE) {
-#pragma unroll
-        for (int x = 0; x < NA; ++x)
-#pragma unroll
-            for (int y = 0; y < NCW; ++y)
-                *reinterpret_cast<f32x4 *>(slots + (int64_t)(seg + 1) * (DA * DC) + ((x * NCW + y) * 256 + tid) * 4) = S[x][y];
+        float *const own = slots + (seg + 1) * state_n;
+        each_state([&](float v, bool in, int64_t at) { if (in) own[at] = v; return v; });
         return;
     }
     // ---- rows behind the sequence are zero; the last segment ends with the state behind the whole sequence
@@ -395,75 +393,38 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
         if (p.out_f32) static_cast<float *>(p.out)[at] = 0.f;
         else static_cast<T *>(p.out)[at] = T(0);
     }
-    if (p.s_fin && seg == p.nseg - 1)
-#pragma unroll
-        for (int x = 0; x < NA; ++x)
-#pragma unroll
-            for (int y = 0; y < NCW; ++y) {
-                const int a = 16 * (a_t0 + x) + 4 * g, c = 16 * (c_t0 + y) + l;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (a + i < p.da && c < dcw) p.s_fin[st_base + (a + i) * p.s_a + (c0 + c) * p.s_c] = S[x][y][i];
-            }
+    if (p.s_fin && seg == p.nseg - 1) each_state([&](float v, bool in, int64_t at) { if (in) p.s_fin[st_base + at] = v; return v; });
 }
 
-// States the segments start from: slot s + 1 holds segment s's own state, slot s receives
-//     start_{s+1} = e^{g cnt_s} start_s + own_s,    start_0 = s_in
-// (start_0 as well: the last segment may write its final state over s_in while the first one runs). One thread per four accumulator values
-// of k_decay_chunk, the same place in every slot.
-template <int DA, int DC> __global__ __launch_bounds__(256) void k_decay_scan(DecayPass p, int ndc) {
-    constexpr int NA = DA >= 64 ? DA / 64 : 1, NC = DC / 16, NCW = DA >= 64 ? NC : NC / 2;
-    const int vec = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x, nh = tile / ndc, c0 = tile % ndc * DC, n = nh / p.H, h = nh % p.H;
-    const int len = p.lengths ? min(max(p.lengths[n], 0), p.T) : p.T;
-    const float gl = p.log_decay[h];
-    const int x = vec / NCW, y = vec % NCW;
-    const int a = 16 * ((DA >= 64 ? w * NA : w & 1) + x) + 4 * g, c = 16 * ((DA >= 64 ? 0 : (w >> 1) * NCW) + y) + l;
-    f32x4 S = {0.f, 0.f, 0.f, 0.f};
-    if (p.s_in)
-        for (int i = 0; i < 4; ++i)
-            if (a + i < p.da && c0 + c < p.dc) S[i] = p.s_in[(int64_t)nh * p.da * p.dc + (a + i) * p.s_a + (c0 + c) * p.s_c];
-    f32x4 *slot = reinterpret_cast<f32x4 *>(p.seg) + (int64_t)tile * p.nseg * (DA * DC / 4) + vec * 256 + tid;
-    slot[0] = S;
-#pragma unroll 8
-    for (int s = 1; s < p.nseg; ++s) {
-        const int cnt = min(max(len - (s - 1) * p.seg_len, 0), p.seg_len);
-        const float keep = cnt == 0 ? 1.f : expf(gl * (float)cnt);
-        const f32x4 own = slot[(int64_t)s * (DA * DC / 4)];
-        for (int i = 0; i < 4; ++i) S[i] = keep * S[i] + own[i];
-        slot[(int64_t)s * (DA * DC / 4)] = S;
-    }
-}
-
-template <typename T, int DA, int DC, bool VEC> int launch(const DecayPass &p, const DecayPlan &pl, hipStream_t st) {
-    typedef Lds<T, DA, DC> L;
-    static_assert(L::BYTES <= kMaxLds, "LDS of one CU");
-    const int64_t tiles = (int64_t)p.n * p.H * pl.ndc;
-    EVFLY_REQUIRE(tiles * pl.nseg <= INT32_MAX, "decay_attention: %lld tiles of work", (long long)(tiles * pl.nseg));
+template <typename T, int DA, int DC, bool VEC, bool STATE> int launch(const DecayPasses &ps, hipStream_t st) {
+    constexpr int bytes = STATE ? Lds<T, DA, DC>::STATE_BYTES : Lds<T, DA, DC>::BYTES;
+    static_assert(bytes <= kMaxLds, "LDS of one CU");
+    const DecayPass &p = ps.p[0];
+    const int64_t blocks = (int64_t)p.n * p.H * ((p.dc + DC - 1) / DC) * (STATE ? p.nseg - 1 : p.nseg) * ps.np;
+    EVFLY_REQUIRE(blocks <= INT32_MAX, "decay_attention: %lld tiles of work", (long long)blocks);
+    const auto kern = k_decay_chunk<T, DA, DC, VEC, STATE>;
     static std::atomic<bool> attr_set[64];
     int dev = 0;
     EVFLY_HIP(hipGetDevice(&dev));
     EVFLY_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
     if (!attr_set[dev].load(std::memory_order_acquire)) {
-        EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_decay_chunk<T, DA, DC, VEC, false>), hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES));
-        EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_decay_chunk<T, DA, DC, VEC, true>), hipFuncAttributeMaxDynamicSharedMemorySize, L::STATE_BYTES));
+        EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         attr_set[dev].store(true, std::memory_order_release);
     }
-    if (pl.nseg > 1) {
-        hipLaunchKernelGGL((k_decay_chunk<T, DA, DC, VEC, true>), dim3((unsigned)(tiles * (pl.nseg - 1))), dim3(256), L::STATE_BYTES, st, p, pl.ndc);
-        hipLaunchKernelGGL((k_decay_scan<DA, DC>), dim3((unsigned)tiles, DA * DC / 1024), dim3(256), 0, st, p, pl.ndc);
-    }
-    hipLaunchKernelGGL((k_decay_chunk<T, DA, DC, VEC, false>), dim3((unsigned)(tiles * pl.nseg)), dim3(256), L::BYTES, st, p, pl.ndc);
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), bytes, st, ps);
     EVFLY_LAUNCH_CHECK();
     return 0;
 }
 
-template <typename T, int DA, int DC> int launch_v(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st) {
-    return vec ? launch<T, DA, DC, true>(p, pl, st) : launch<T, DA, DC, false>(p, pl, st);
+template <typename T, int DA, int DC> int launch_v(const DecayPasses &p, bool state, bool vec, hipStream_t st) {
+    if (state) return vec ? launch<T, DA, DC, true, true>(p, st) : launch<T, DA, DC, false, true>(p, st);
+    return vec ? launch<T, DA, DC, true, false>(p, st) : launch<T, DA, DC, false, false>(p, st);
 }
-template <typename T> int launch_all(const DecayPass &p, const DecayPlan &pl, bool vec, hipStream_t st) {
-    if (pl.DC == 32) return pl.DA == 32 ? launch_v<T, 32, 32>(p, pl, vec, st) : pl.DA == 64 ? launch_v<T, 64, 32>(p, pl, vec, st) : launch_v<T, 128, 32>(p, pl, vec, st);
-    return pl.DA == 32 ? launch_v<T, 32, 64>(p, pl, vec, st) : pl.DA == 64 ? launch_v<T, 64, 64>(p, pl, vec, st) : launch_v<T, 128, 64>(p, pl, vec, st);
+template <typename T> int launch_all(const DecayPasses &p, bool state, bool vec, hipStream_t st) {
+    const int DA = decay_tile_a(p.p[0].da);
+    if (decay_tile_c(p.p[0].dc) == 32)
+        return DA == 32 ? launch_v<T, 32, 32>(p, state, vec, st) : DA == 64 ? launch_v<T, 64, 32>(p, state, vec, st) : launch_v<T, 128, 32>(p, state, vec, st);
+    return DA == 32 ? launch_v<T, 32, 64>(p, state, vec, st) : DA == 64 ? launch_v<T, 64, 64>(p, state, vec, st) : launch_v<T, 128, 64>(p, state, vec, st);
 }
 
 }  // namespace decay
