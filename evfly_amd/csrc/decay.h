@@ -36,7 +36,7 @@ struct DecayPasses {
 
 // Split of the sequence into segments that run side by side.
 struct DecaySplit { int nseg, seg_len; };
-DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype);
+DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype, bool backward);
 
 // All passes have the same da and dc classes. STATE: the segments' own states only (into slot segment + 1 of seg), no output.
 int decay_passes_f32(const DecayPasses &p, bool state, bool vec, hipStream_t st);

@@ -214,7 +214,7 @@ Ws decay_ws(int n, int T, int H, int KV, int dk, int dv, int dtype, bool backwar
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
     Ws w{0, 0, 0, 0};
     if (T > EVFLY_DECAY_STEP_TOKENS || backward) {
-        const DecaySplit sp = decay_split(n, T, H, dk, dv, dtype);
+        const DecaySplit sp = decay_split(n, T, H, dk, dv, dtype, backward);
         if (sp.nseg > 1) w.seg_floats = up((int64_t)n * H * sp.nseg * dk * dv * 4) / 4;
     }
     w.part_k = w.seg_floats * 4 * (backward ? 2 : 1);
@@ -240,19 +240,44 @@ void token_strides(const int64_t *s, int T, int heads, int d, int64_t (&out)[3])
 
 }  // namespace
 
-// The sequence is cut where there are fewer than four blocks per CU, into pieces of at least four chunks: a cut costs two of the four token tensors a
-// second read and the state a round trip.
-DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype) {
-    const int64_t base = (int64_t)n * H * ((dv + decay_tile_c(dv) - 1) / decay_tile_c(dv));
-    int64_t nseg = base > 0 ? (4 * kNumCU + base - 1) / base : 1;
-    const int64_t most = (T + 4 * DECAY_CHUNK - 1) / (4 * DECAY_CHUNK);
-    nseg = nseg < most ? nseg : most;
-    nseg = nseg > 1 ? nseg : 1;
-    int64_t len = (T + nseg - 1) / nseg;
-    len = (len + DECAY_CHUNK - 1) / DECAY_CHUNK * DECAY_CHUNK;
-    if (len < DECAY_CHUNK) len = DECAY_CHUNK;
-    nseg = (T + len - 1) / len;
-    return DecaySplit{(int)(nseg > 1 ? nseg : 1), (int)len};
+// Segments of a sequence. More of them fill the CUs and shorten the longest chain of chunks, but each cut makes two of the token tensors read twice (the state
+// pass, 0.4 of a chunk's work) and adds two launches. The split with the smallest estimate is taken:
+//     chunks per segment * t * max(1, share * blocks per CU), for each launch of the pass and, at 0.4 t, for the state pass, plus 10 us if it is cut at all
+// with t the time of a lone block's chunk (by type and a dimension) and `share` what a block uses of its CU. Measured against sweeps of 1 .. 16 blocks per CU on
+// eleven shapes; us forward / backward, chosen and the neighbours: 8 x 4096 x 16 heads x 64 bf16, four segments 96 forward (two 132, eight 105), two
+// 203 backward (four 213, eight 226); 16 x 2048 x 16 x 64 bf16, one 91 / 156 (two 97 / 198); 6 x 500 x 8 x 40 / 72 fp32, eight 35 / 89 (four 40 / 97, two 46 / 98);
+// 64 x 300 x 8 x 64 bf16, one 25 / 47 (two 45 / 86).
+namespace {
+int col_tiles(int c) { return (c + decay_tile_c(c) - 1) / decay_tile_c(c); }
+// the gradients' passes have their roles exchanged: one launch serves all three if both head sizes have the same tiles
+bool decay_one_launch(int dk, int dv) {
+    return decay_tile_a(dk) == decay_tile_a(dv) && decay_tile_c(dk) == decay_tile_c(dv) && col_tiles(dk) == col_tiles(dv);
+}
+}  // namespace
+DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype, bool backward) {
+    const bool f32 = dtype == EVFLY_DTYPE_F32;
+    const double rows = (double)n * H, share = f32 ? 0.7 : 0.8;
+    const int chunks = (T + DECAY_CHUNK - 1) / DECAY_CHUNK;
+    auto launch_cost = [&](int a, double blocks) {
+        const int DA = decay_tile_a(a);
+        const double busy = std::ceil(blocks / kNumCU) * share;
+        return (f32 ? 4.0 : 2.5) * (DA == 128 ? 1.7 : DA == 64 ? 1.0 : 0.6) * (busy > 1.0 ? busy : 1.0);
+    };
+    DecaySplit best{1, DECAY_CHUNK * (chunks > 0 ? chunks : 1)};
+    double least = INFINITY;
+    for (int want = 1; want <= chunks && (want == 1 || rows * want <= 16 * kNumCU); want += want < 4 ? 1 : want / 4) {
+        const int per = (chunks + want - 1) / want, nseg = (chunks + per - 1) / per;
+        double cost;
+        if (!backward) cost = launch_cost(dk, rows * nseg * col_tiles(dv));
+        else if (decay_one_launch(dk, dv)) cost = launch_cost(dk, rows * nseg * col_tiles(dv) * 3);
+        else cost = launch_cost(dv, rows * nseg * col_tiles(dk) * 2) + launch_cost(dk, rows * nseg * col_tiles(dv));
+        if (nseg > 1) cost += 0.4 * launch_cost(dk, rows * (nseg - 1) * col_tiles(dv) * (backward ? 2 : 1)) + 10.0 / per;
+        if (cost * per < 0.99 * least) {
+            least = cost * per;
+            best = DecaySplit{nseg, per * DECAY_CHUNK};
+        }
+    }
+    return best;
 }
 
 }  // namespace evfly
@@ -291,7 +316,7 @@ extern "C" int evfly_decay_attention_forward(const void *q, const void *k, const
     }
     const int vec = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
     Run run{dtype, vec_ok(tq, vec) && vec_ok(tk, vec) && vec_ok(tv, vec) && aligned16(out), st, DecayPass{}};
-    const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype);
+    const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype, false);
     DecayPass &b = run.base;
     b.log_decay = log_decay; b.lengths = lengths; b.n = n_streams; b.T = tokens; b.H = heads; b.nseg = sp.nseg; b.seg_len = sp.seg_len;
     b.seg = static_cast<float *>(workspace); b.s_in = state_in; b.s_a = dv; b.s_c = 1;
@@ -325,7 +350,7 @@ extern "C" int evfly_decay_attention_backward(const void *q, const void *k, cons
     EVFLY_REQUIRE(!d_state_in || d_state_in != d_state_out, "decay_attention_backward: d_state_in is d_state_out");
     const int vec = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
     Run run{dtype, vec_ok(tq, vec) && vec_ok(tk, vec) && vec_ok(tv, vec) && vec_ok(to, vec) && aligned16(dq) && aligned16(dk_out) && aligned16(dv_out), st, DecayPass{}};
-    const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype);
+    const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype, true);
     char *const w = static_cast<char *>(workspace);
     float *const seg = reinterpret_cast<float *>(w), *const part_k = reinterpret_cast<float *>(w + ws.part_k), *const part_v = reinterpret_cast<float *>(w + ws.part_v);
     DecayPass &b = run.base;
@@ -351,7 +376,7 @@ extern "C" int evfly_decay_attention_backward(const void *q, const void *k, cons
     }
     DecayPasses ps{};
     ps.p[0] = pq; ps.p[1] = pk; ps.p[2] = pv;
-    if (decay_tile_a(dk) == decay_tile_a(dv) && decay_tile_c(dk) == decay_tile_c(dv) && (dk + decay_tile_c(dk) - 1) / decay_tile_c(dk) == (dv + decay_tile_c(dv) - 1) / decay_tile_c(dv)) {
+    if (decay_one_launch(dk, dv)) {
         ps.np = 3;
         if (int rc = run.launch(ps, false)) return rc;
     } else {
