@@ -123,10 +123,17 @@ def load_library():
     return _LIB
 
 
+_GPU_SEEN = False
+
+
 def lib():
-    """The library, for compute: additionally requires a visible GPU."""
+    """The library, for compute: additionally requires a visible GPU (looked for until one was seen)."""
+    global _GPU_SEEN
+    if _GPU_SEEN:
+        return load_library()
     import torch
-    if not torch.cuda.is_available():
+    _GPU_SEEN = torch.cuda.is_available()
+    if not _GPU_SEEN:
         raise RuntimeError("evfly_amd: no MI355X/ROCm device visible; the HIP path is the only path "
                            "(there is no CPU fallback).")
     return load_library()

@@ -13,7 +13,6 @@ import ctypes as C
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -24,24 +23,29 @@ STEP_TOKENS = 16                    # up to here a forward needs no workspace (E
 _NORM = {None: 0, "layer": 1, "rms": 2}
 
 
-class _on:
-    """`with torch.cuda.device(t.device)` that costs nothing where the device is the current one (the usual case)."""
-
-    def __init__(self, t):
-        self.prev = torch.cuda.current_device()
-        self.dev = t.device.index
-
-    def __enter__(self):
-        if self.dev != self.prev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.dev != self.prev:
-            torch.cuda.set_device(self.prev)
+_getDevice, _rawStream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream      # (a tick's call is a few microseconds: no Stream object for it)
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _dense(t):
+    return None if t is None else t.contiguous()
+
+
+def _on_its_device(fn):
+    """`fn(t, ...)` with t's device as the current one (it usually is)."""
+    def call(t, *args):
+        if t.get_device() == _getDevice():
+            return fn(t, *args)
+        with torch.cuda.device(t.device):
+            return fn(t, *args)
+    return call
+
+
+def _workspace(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes > 0 else None
 
 
 def _check_tokens(who, named, like):
@@ -61,15 +65,29 @@ def _check_f32(who, name, t, shape, device):
 
 
 # ---------------------------------------------------------------------------------------- decay attention
-def _check_decay(who, q, k, v, log_decay, state, lengths, scale):
-    _lib.lib()                                                   # (no GPU / no library: that error first)
+def _decay_fits(q, k, v, log_decay, state, lengths, lead):
+    """Everything `_refuse_decay` asks for, in one look."""
+    try:
+        dt, dev, qs, ks, vs = q.dtype, q.device, q.shape, k.shape, v.shape
+        H, KV, dk, dv = qs[-2], ks[-2], qs[-1], vs[-1]
+        return (len(qs) == lead + 2 and dt in _DTYPE and k.dtype is dt and v.dtype is dt and dev.type == "cuda" and k.device == dev and v.device == dev and
+                ks[:lead] == qs[:lead] and vs[:lead] == qs[:lead] and ks[-1] == dk and vs[-2] == KV and KV > 0 and H > 0 and H % KV == 0 and
+                0 < dk <= MAX_HEAD_DIM and 0 < dv <= MAX_HEAD_DIM and
+                log_decay.dtype is torch.float32 and log_decay.shape == (H,) and log_decay.device == dev and not log_decay.requires_grad and
+                (state is None or (state.dtype is torch.float32 and state.shape == (qs[0], H, dk, dv) and state.device == dev)) and
+                (lengths is None or (lengths.dtype is torch.int32 and lengths.shape == qs[:1] and lengths.device == dev)))
+    except (AttributeError, IndexError):
+        return False
+
+
+def _refuse_decay(who, q, k, v, log_decay, state, lengths, lead):
+    sizes = "(streams, tokens, heads, head size)" if lead == 2 else "(streams, heads, head size)"
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(t, torch.Tensor) or t.dim() != 4:
-            raise ValueError(f"{who}: {name} must be a tensor (streams, tokens, heads, head size)")
+        if not isinstance(t, torch.Tensor) or t.dim() != lead + 2:
+            raise ValueError(f"{who}: {name} must be a tensor {sizes}")
     _check_tokens(who, (("q", q), ("k", k), ("v", v)), q)
-    n, T, H, dk = q.shape
-    KV, dv = v.shape[2], v.shape[3]
-    if tuple(k.shape) != (n, T, KV, dk) or tuple(v.shape[:2]) != (n, T):
+    H, KV, dk, dv = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
+    if k.shape[:lead] != q.shape[:lead] or v.shape[:lead] != q.shape[:lead] or k.shape[-1] != dk or v.shape[-2] != KV:
         raise ValueError(f"{who}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
     if KV == 0 or H == 0 or H % KV:
         raise ValueError(f"{who}: {H} heads do not share {KV} key / value heads evenly")
@@ -79,11 +97,17 @@ def _check_decay(who, q, k, v, log_decay, state, lengths, scale):
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{who}: log_decay is a constant of the head and has no gradient (detach it)")
     if state is not None:
-        _check_f32(who, "state", state, (n, H, dk, dv), q.device)
-    if lengths is not None and (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or tuple(lengths.shape) != (n,)
+        _check_f32(who, "state", state, (q.shape[0], H, dk, dv), q.device)
+    if lengths is not None and (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],)
                                 or lengths.device != q.device):
-        raise ValueError(f"{who}: lengths must be an int32 tensor ({n},) on {q.device}")
-    scale = dk ** -0.5 if scale is None else float(scale)
+        raise ValueError(f"{who}: lengths must be an int32 tensor ({q.shape[0]},) on {q.device}")
+
+
+def _check_decay(who, q, k, v, log_decay, state, lengths, scale, lead):
+    _lib.lib()                                                   # (no GPU / no library: that error first)
+    if not _decay_fits(q, k, v, log_decay, state, lengths, lead):
+        _refuse_decay(who, q, k, v, log_decay, state, lengths, lead)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{who}: scale is not finite")
     return scale
@@ -97,60 +121,72 @@ def _rows(t):
 def _strides(q, k, v):
     if q.is_contiguous() and k.is_contiguous() and v.is_contiguous():
         return None
+    if q.dim() == 3:                                             # one token: its stride is never taken
+        return (C.c_int64 * 9)(*(s for t in (q, k, v) for s in (t.stride(0), 0, t.stride(1))))
     return (C.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
 
 
+@_on_its_device
 def _decay_forward(q, k, v, log_decay, state, lengths, scale, new_state):
-    n, T, H, dk = q.shape
-    KV, dv = v.shape[2], v.shape[3]
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-    lengths = lengths.contiguous() if lengths is not None else None
+    n, H, dk, KV, dv = q.shape[0], q.shape[-2], q.shape[-1], k.shape[-2], v.shape[-1]
+    T = q.shape[1] if q.dim() == 4 else 1
+    q, k, v, log_decay, state, lengths = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), _dense(state), _dense(lengths)
     dt = _DTYPE[q.dtype]
     L = _lib.load_library()
-    with _on(q):
-        out = torch.empty((n, T, H, dv), dtype=q.dtype, device=q.device)
-        nb = 0 if T <= STEP_TOKENS else _lib.check(L.evfly_decay_attention_workspace_bytes(n, T, H, KV, dk, dv, dt, 0))
-        ws = _workspace(nb, q.device)
-        _lib.check(L.evfly_decay_attention_forward(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), log_decay.data_ptr(), _lib.ptr(state), _lib.ptr(lengths),
-            n, T, H, KV, dk, dv, scale, dt, out.data_ptr(), _lib.ptr(new_state), _lib.ptr(ws), nb, _lib.cur_stream()))
+    out = torch.empty((*q.shape[:-1], dv), dtype=q.dtype, device=q.device)
+    nb, ws = 0, None
+    if T > STEP_TOKENS:
+        nb = _lib.check(L.evfly_decay_attention_workspace_bytes(n, T, H, KV, dk, dv, dt, 0))
+        ws = _workspace(nb, q)
+    _lib.check(L.evfly_decay_attention_forward(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), log_decay.data_ptr(), _ptr(state), _ptr(lengths), n, T, H, KV, dk, dv, scale, dt,
+        out.data_ptr(), new_state.data_ptr(), _ptr(ws), nb, _rawStream(q.get_device())))
     return out
+
+
+@_on_its_device
+def _decay_backward(q, k, v, log_decay, state, lengths, scale, d_out, d_state, want_state):
+    n, T, H, dk = q.shape
+    KV, dv = v.shape[2], v.shape[3]
+    dt = _DTYPE[q.dtype]
+    L = _lib.load_library()
+    d_out = torch.zeros((n, T, H, dv), dtype=q.dtype, device=q.device) if d_out is None else d_out.contiguous()
+    dq, dk_, dv_ = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    q, k, v, log_decay, state, lengths, d_state = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), _dense(state), _dense(lengths), _dense(d_state)
+    ds = torch.empty_like(state) if want_state else None
+    nb = _lib.check(L.evfly_decay_attention_workspace_bytes(n, T, H, KV, dk, dv, dt, 1))
+    ws = _workspace(nb, q)
+    _lib.check(L.evfly_decay_attention_backward(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), log_decay.data_ptr(), _ptr(state), _ptr(lengths), d_out.data_ptr(), _ptr(d_state),
+        n, T, H, KV, dk, dv, scale, dt, dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(), _ptr(ds), _ptr(ws), nb, _rawStream(q.get_device())))
+    return dq, dk_, dv_, ds
+
+
+def _new_state(q, v):
+    return torch.empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+
+
+def _no_second_order(who):
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{who}: its gradients have no gradients (create_graph=True)")
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, lengths, scale):
         ctx.set_materialize_grads(False)
-        n, T, H, dk = q.shape
-        new_state = torch.empty((n, H, dk, v.shape[3]), dtype=torch.float32, device=q.device)
-        out = _decay_forward(q, k, v, log_decay, state.contiguous() if state is not None else None, lengths, scale, new_state)
+        new_state = _new_state(q, v)
+        out = _decay_forward(q, k, v, log_decay, state, lengths, scale, new_state)
         ctx.save_for_backward(q, k, v, log_decay, state, lengths)
         ctx.scale = scale
         return out, new_state
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out, d_state):
+        _no_second_order("decay_attention")
         q, k, v, log_decay, state, lengths = ctx.saved_tensors
-        n, T, H, dk = q.shape
-        KV, dv = v.shape[2], v.shape[3]
-        dt = _DTYPE[q.dtype]
-        L = _lib.load_library()
-        with _on(q):
-            d_out = torch.zeros((n, T, H, dv), dtype=q.dtype, device=q.device) if d_out is None else d_out.contiguous()
-            d_state = d_state.contiguous() if d_state is not None else None
-            qr, kr, vr, g = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-            s_in = state.contiguous() if state is not None else None
-            ln = lengths.contiguous() if lengths is not None else None
-            dq, dk_, dv_ = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-            ds = torch.empty((n, H, dk, dv), dtype=torch.float32, device=q.device) if state is not None and ctx.needs_input_grad[4] else None
-            nb = _lib.check(L.evfly_decay_attention_workspace_bytes(n, T, H, KV, dk, dv, dt, 1))
-            ws = _workspace(nb, q.device)
-            _lib.check(L.evfly_decay_attention_backward(
-                qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), _strides(qr, kr, vr), g.data_ptr(), _lib.ptr(s_in), _lib.ptr(ln), d_out.data_ptr(),
-                _lib.ptr(d_state), n, T, H, KV, dk, dv, ctx.scale, dt, dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(), _lib.ptr(ds),
-                _lib.ptr(ws), nb, _lib.cur_stream()))
-        return dq, dk_, dv_, None, ds, None, None
+        dq, dk, dv, ds = _decay_backward(q, k, v, log_decay, state, lengths, ctx.scale, d_out, d_state, ctx.needs_input_grad[4])
+        return dq, dk, dv, None, ds, None, None
 
 
 def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
@@ -162,12 +198,11 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     -inf nothing); a constant, without a gradient. state (streams, heads, dk, dv) float32 from the call before, None = zeros.
     lengths (streams,) int32: tokens of each stream that are there, None = all; the others are not read, `out` is zero there.
     scale: dk ** -0.5 if None. Returns (out (streams, tokens, heads, dv), new state). Gradients to q, k, v and state."""
-    scale = _check_decay("decay_attention", q, k, v, log_decay, state, lengths, scale)
+    scale = _check_decay("decay_attention", q, k, v, log_decay, state, lengths, scale, 2)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         return _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale)
-    n, T, H, dk = q.shape
-    new_state = torch.empty((n, H, dk, v.shape[3]), dtype=torch.float32, device=q.device)
-    return _decay_forward(q, k, v, log_decay, state.contiguous() if state is not None else None, lengths, scale, new_state), new_state
+    new_state = _new_state(q, v)
+    return _decay_forward(q, k, v, log_decay, state, lengths, scale, new_state), new_state
 
 
 def decay_attention_step(q, k, v, log_decay, state, lengths=None, scale=None, new_state=None):
@@ -175,24 +210,21 @@ def decay_attention_step(q, k, v, log_decay, state, lengths=None, scale=None, ne
     against `state` (streams, heads, dk, dv) float32, contiguous, which is updated in place -- or left as it is, with the new state
     written to `new_state` (a pair of buffers used in turn). lengths (streams,) int32: 0 = no token for this stream in this call (its state
     stays, its row of the result is zero). Returns out (streams, heads, dv). No gradients: use `decay_attention` for them."""
-    if not all(isinstance(t, torch.Tensor) and t.dim() == 3 for t in (q, k, v)):
-        _lib.lib()
-        raise ValueError("decay_attention_step: q, k and v must be tensors (streams, heads, head size)")
-    q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
-    scale = _check_decay("decay_attention_step", q, k, v, log_decay, state, lengths, scale)
+    who = "decay_attention_step"
+    scale = _check_decay(who, q, k, v, log_decay, state, lengths, scale, 1)
     if state is None or not state.is_contiguous():
-        raise ValueError("decay_attention_step: state must be a contiguous tensor")
+        raise ValueError(f"{who}: state must be a contiguous tensor")
     dst = state
     if new_state is not None:
-        _check_f32("decay_attention_step", "new_state", new_state, state.shape, q.device)
+        _check_f32(who, "new_state", new_state, state.shape, q.device)
         if not new_state.is_contiguous():
-            raise ValueError("decay_attention_step: new_state must be a contiguous tensor")
+            raise ValueError(f"{who}: new_state must be a contiguous tensor")
         dst = new_state
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state, dst)):
-        raise ValueError("decay_attention_step has no gradients: call decay_attention, or wrap the call in torch.no_grad()")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or dst.requires_grad):
+        raise ValueError(f"{who} has no gradients: call decay_attention, or wrap the call in torch.no_grad()")
     out = _decay_forward(q, k, v, log_decay, state, lengths, scale, dst)
     torch.autograd.graph.increment_version(dst)                  # written behind autograd's back
-    return out[:, 0]
+    return out
 
 
 # ---------------------------------------------------------------------------------------- block norm
@@ -210,25 +242,44 @@ def _gate_rows(f, gate):
                      f"dimension and 1 from there on)")
 
 
-def _block_args(f, x, gate, res_scale, vecs, opt):
-    gate_f32 = gate is not None and gate.dtype == torch.float32
-    return (f.data_ptr(), _lib.ptr(x), _lib.ptr(gate), opt["rows_per_gate"], int(gate_f32), opt["act"], _lib.ptr(res_scale), opt["post"],
-            _lib.ptr(vecs[0]), _lib.ptr(vecs[1]), opt["pre"], _lib.ptr(vecs[2]), _lib.ptr(vecs[3]), opt["eps"])
-
-
-def _block_forward(f, x, gate, res_scale, vecs, opt):
+@_on_its_device
+def _block_forward(f, x, gate, res_scale, w1, b1, w2, b2, opt):
+    rows_per_gate, gate_f32, act, post, pre, eps = opt
+    f, x, gate, res_scale, w1, b1, w2, b2 = f.contiguous(), _dense(x), _dense(gate), _dense(res_scale), _dense(w1), _dense(b1), _dense(w2), _dense(b2)
     Cn = f.shape[-1]
-    rows = f.numel() // Cn
-    with _on(f):
-        y = torch.empty(f.shape, dtype=f.dtype, device=f.device)
-        h = torch.empty(f.shape, dtype=f.dtype, device=f.device) if opt["pre"] else None
-        _lib.check(_lib.load_library().evfly_block_norm_forward(*_block_args(f, x, gate, res_scale, vecs, opt), rows, Cn, _DTYPE[f.dtype],
-                                                                y.data_ptr(), _lib.ptr(h), _lib.cur_stream()))
+    y = torch.empty_like(f)
+    h = torch.empty_like(f) if pre else None
+    _lib.check(_lib.load_library().evfly_block_norm_forward(
+        f.data_ptr(), _ptr(x), _ptr(gate), rows_per_gate, gate_f32, act, _ptr(res_scale), post, _ptr(w1), _ptr(b1), pre, _ptr(w2), _ptr(b2), eps,
+        f.numel() // Cn, Cn, _DTYPE[f.dtype], y.data_ptr(), _ptr(h), _rawStream(f.get_device())))
     return y, h
 
 
-def _dense(t):
-    return t.contiguous() if t is not None else None
+@_on_its_device
+def _block_backward(f, x, gate, res_scale, w1, b1, w2, b2, opt, dy, dh, need):
+    rows_per_gate, gate_f32, act, post, pre, eps = opt
+    f, x, gate, res_scale, w1, b1, w2, b2, dy, dh = (f.contiguous(), _dense(x), _dense(gate), _dense(res_scale), _dense(w1), _dense(b1), _dense(w2), _dense(b2),
+                                                     _dense(dy), _dense(dh))
+    Cn = f.shape[-1]
+    rows, dt = f.numel() // Cn, _DTYPE[f.dtype]
+    L = _lib.load_library()
+    # f's gradient is always formed; of the others what is asked for, the vectors as rows of one tensor
+    df = torch.empty_like(f)
+    dx = torch.empty_like(x) if x is not None and need[1] else None
+    dg = torch.empty_like(gate) if gate is not None and need[2] else None
+    if dg is not None and rows == 0:
+        dg.zero_()
+    vec = [None] * 5
+    ask = [i for i, t in enumerate((res_scale, w1, b1, w2, b2)) if t is not None and need[3 + i]]
+    if ask:
+        for i, t in zip(ask, torch.empty((len(ask), Cn), dtype=torch.float32, device=f.device).unbind(0)):
+            vec[i] = t
+    nb = _lib.check(L.evfly_block_norm_workspace_bytes(rows, Cn, rows_per_gate, dt))
+    ws = _workspace(nb, f)
+    _lib.check(L.evfly_block_norm_backward(
+        f.data_ptr(), _ptr(x), _ptr(gate), rows_per_gate, gate_f32, act, _ptr(res_scale), post, _ptr(w1), _ptr(b1), pre, _ptr(w2), _ptr(b2), eps, _ptr(dy),
+        _ptr(dh), rows, Cn, dt, df.data_ptr(), _ptr(dx), _ptr(dg), *map(_ptr, vec), _ptr(ws), nb, _rawStream(f.get_device())))
+    return (df if need[0] else None, dx, dg, *vec, None)
 
 
 class _BlockNorm(torch.autograd.Function):
@@ -237,31 +288,13 @@ class _BlockNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(f, x, gate, res_scale, w1, b1, w2, b2)
         ctx.opt = opt
-        y, h = _block_forward(_dense(f), _dense(x), _dense(gate), _dense(res_scale), [_dense(t) for t in (w1, b1, w2, b2)], opt)
+        y, h = _block_forward(f, x, gate, res_scale, w1, b1, w2, b2, opt)
         return (y, h) if h is not None else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
-        opt, need = ctx.opt, ctx.needs_input_grad
-        ins = [_dense(t) for t in ctx.saved_tensors]
-        f, x, gate = ins[:3]
-        Cn = f.shape[-1]
-        rows = f.numel() // Cn
-        L = _lib.load_library()
-        with _on(f):
-            dy, dh = _dense(dy), _dense(dh)
-            # f's gradient is always formed; of the others what was asked for. (no rows: the kernels write the vectors' zeros, a gate's come from here)
-            g = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and (i == 0 or need[i]) else None
-                 for i, t in enumerate(ins)]
-            if rows == 0 and g[2] is not None:
-                g[2].zero_()
-            nb = _lib.check(L.evfly_block_norm_workspace_bytes(rows, Cn, opt["rows_per_gate"], _DTYPE[f.dtype]))
-            ws = _workspace(nb, f.device)
-            _lib.check(L.evfly_block_norm_backward(*_block_args(f, x, gate, ins[3], ins[4:], opt), _lib.ptr(dy), _lib.ptr(dh), rows, Cn, _DTYPE[f.dtype],
-                                                   g[0].data_ptr(), _lib.ptr(g[1]), _lib.ptr(g[2]), _lib.ptr(g[3]), _lib.ptr(g[4]), _lib.ptr(g[5]),
-                                                   _lib.ptr(g[6]), _lib.ptr(g[7]), _lib.ptr(ws), nb, _lib.cur_stream()))
-        return (*[t if need[i] else None for i, t in enumerate(g)], None)
+        _no_second_order("block_norm")
+        return _block_backward(*ctx.saved_tensors, ctx.opt, dy, dh, ctx.needs_input_grad)
 
 
 def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None, post_weight=None, post_bias=None,
@@ -276,8 +309,9 @@ def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None,
     _lib.lib()
     if not isinstance(f, torch.Tensor) or f.dim() < 1 or not 1 <= f.shape[-1] <= MAX_CHANNELS:
         raise ValueError(f"block_norm: f must be a tensor (..., channels) of 1 .. {MAX_CHANNELS} channels")
-    _check_tokens("block_norm", (("f", f),) if x is None else (("f", f), ("x", x)), f)
-    Cn = f.shape[-1]
+    dt, dev, vec = f.dtype, f.device, f.shape[-1:]
+    if dt not in _DTYPE or dev.type != "cuda" or (x is not None and not (isinstance(x, torch.Tensor) and x.dtype is dt and x.device == dev)):
+        _check_tokens("block_norm", (("f", f),) if x is None else (("f", f), ("x", x)), f)
     if x is not None and x.shape != f.shape:
         raise ValueError(f"block_norm: x {tuple(x.shape)} is not shaped like f {tuple(f.shape)}")
     if post not in _NORM or pre not in _NORM:
@@ -289,7 +323,8 @@ def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None,
         if t is not None:
             if not kind:
                 raise ValueError(f"block_norm: {name} without a norm")
-            _check_f32("block_norm", name, t, (Cn,), f.device)
+            if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == vec and t.device == dev):
+                _check_f32("block_norm", name, t, vec, dev)
     if gate_act not in ("none", "sigmoid", "tanh"):
         raise ValueError(f"block_norm: gate_act {gate_act!r} (\"none\", \"sigmoid\" or \"tanh\")")
     eps = float(eps)
@@ -300,9 +335,10 @@ def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None,
         if not isinstance(gate, torch.Tensor) or gate.dtype not in (f.dtype, torch.float32) or gate.device != f.device:
             raise ValueError(f"block_norm: gate must be a {f.dtype} or float32 tensor on {f.device}")
         rows_per_gate = max(1, _gate_rows(f, gate))
-    opt = dict(rows_per_gate=rows_per_gate, act=_lib.ACT_CODES[gate_act], post=_NORM[post], pre=_NORM[pre], eps=eps)
-    ins = (f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins):
-        got = _BlockNorm.apply(*ins, opt)
-        return got if isinstance(got, tuple) else (got, None)
-    return _block_forward(*[_dense(t) for t in ins[:4]], [_dense(t) for t in ins[4:]], opt)
+    opt = (rows_per_gate, int(gate is not None and gate.dtype is torch.float32), _lib.ACT_CODES[gate_act], _NORM[post], _NORM[pre], eps)
+    if torch.is_grad_enabled():
+        for t in (f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias):
+            if t is not None and t.requires_grad:
+                got = _BlockNorm.apply(f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias, opt)
+                return got if isinstance(got, tuple) else (got, None)
+    return _block_forward(f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias, opt)
