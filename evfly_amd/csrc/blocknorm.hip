@@ -9,6 +9,7 @@
 // Column sums (weights, biases, residual scale, a broadcast gate) are kept per lane over the block's rows, added over the block's groups in LDS, written
 // as one partial row per block and added in block order by k_bn_columns: no atomics, the same bits on every call.
 #include <cmath>
+#include <type_traits>
 
 #include "bf16.h"
 #include "common.h"
@@ -37,29 +38,34 @@ struct BnArgs {
 };
 enum { K_ALPHA, K_W1, K_B1, K_W2, K_B2, K_GATE, K_N };
 
-// A lane's eight values are E / W pieces of W neighbouring ones: value j lies in column ((j / W) G + gl) W + j % W. Columns behind C read as zero.
-template <typename S, int W, int G> __device__ __forceinline__ void load_row(const S *row, int gl, int C, float (&v)[E]) {
-    constexpr int VS = 16 / sizeof(S);
+// A lane's eight values are E / W pieces of W neighbouring ones: value j lies in column ((j / W) G + gl) W + j % W. Columns behind C read as zero. A row is
+// fetched as it lies in memory (one row ahead of its use) and widened when its turn comes.
+template <typename S, int W, int G> struct Row {
+    static constexpr int VS = W == 1 ? 1 : 16 / sizeof(S);               // values per load
+    typename std::conditional<W == 1, S, uint4>::type raw[E / VS];
+    __device__ __forceinline__ void fetch(const S *row, int gl, int C) {
 #pragma unroll
-    for (int j = 0; j < E / W; ++j) {
-        const int c = (j * G + gl) * W;
-        if constexpr (W == 1) {
-            v[j] = c < C ? Elem<S>::ld1(row + c) : 0.f;
-        } else {
-#pragma unroll
-            for (int e = 0; e < W; ++e) v[j * W + e] = 0.f;
-            if (c < C) {
-#pragma unroll
-                for (int e = 0; e < W; e += VS) {
-                    float t[VS];
-                    Elem<S>::load(row + c + e, t);
-#pragma unroll
-                    for (int i = 0; i < VS; ++i) v[j * W + e + i] = t[i];
-                }
-            }
+        for (int k = 0; k < E / VS; ++k) {
+            const int c = (k * VS / W * G + gl) * W + k * VS % W;
+            if constexpr (W == 1) raw[k] = c < C ? row[c] : S(0);
+            else raw[k] = c < C ? *reinterpret_cast<const uint4 *>(row + c) : make_uint4(0, 0, 0, 0);
         }
     }
-}
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int k = 0; k < E / VS; ++k) raw[k] = {};
+    }
+    __device__ __forceinline__ void widen(float (&v)[E]) const {
+#pragma unroll
+        for (int k = 0; k < E / VS; ++k) {
+            float t[VS];
+            if constexpr (W == 1) t[0] = Elem<S>::ld1(&raw[k]);
+            else Elem<S>::load(reinterpret_cast<const S *>(&raw[k]), t);
+#pragma unroll
+            for (int i = 0; i < VS; ++i) v[k * VS + i] = t[i];
+        }
+    }
+};
 template <typename S, int W, int G> __device__ __forceinline__ void store_row(S *row, int gl, int C, const float (&v)[E]) {
     constexpr int VS = 16 / sizeof(S);
 #pragma unroll
@@ -92,7 +98,9 @@ template <typename T, int W, int G> __device__ __forceinline__ void load_gate(co
         const float *g = static_cast<const float *>(p.gate) + row * p.C;
         load_vec<W, G>(g, gl, p.C, 0.f, v);
     } else {
-        load_row<T, W, G>(static_cast<const T *>(p.gate) + row * p.C, gl, p.C, v);
+        Row<T, W, G> t;
+        t.fetch(static_cast<const T *>(p.gate) + row * p.C, gl, p.C);
+        t.widen(v);
     }
 }
 // act(z) in place of z; slope = act'(z)
@@ -178,28 +186,36 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
     load_vec<W, G>(p.b2, gl, p.C, 0.f, b2);
     load_vec<W, G>(p.alpha, gl, p.C, 1.f, al);
     int64_t held = -1;                               // gate row in a[]
+    const bool token_gate = p.gate && p.rpg == 1 && !p.gate_f32;
+    Row<T, W, G> nf, nx, ng;
+    nf.clear(); nx.clear(); ng.clear();
+    auto fetch = [&](int64_t r) {
+        if (r >= p.rows) return;
+        nf.fetch(static_cast<const T *>(p.f) + r * p.C, gl, p.C);
+        if (p.x) nx.fetch(static_cast<const T *>(p.x) + r * p.C, gl, p.C);
+        if (token_gate) ng.fetch(static_cast<const T *>(p.gate) + r * p.C, gl, p.C);
+    };
+    fetch((int64_t)blockIdx.x * GR + gi);
     for (int64_t r0 = (int64_t)blockIdx.x * GR; r0 < p.rows; r0 += (int64_t)gridDim.x * GR) {
         const int64_t r = r0 + gi;
         const bool live = r < p.rows;
         float v[E], x[E];
+        nf.widen(v);
+        nx.widen(x);
+        if (p.gate && live) {
+            const int64_t gr = p.rpg == 1 ? r : (uint32_t)r / p.rpg;
+            if (gr != held) {
+                if (token_gate) ng.widen(a);
+                else load_gate<T, W, G>(p, gr, gl, a);
+                held = gr;
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = x[j] = 0.f;
-        if (live) {
-            load_row<T, W, G>(static_cast<const T *>(p.f) + r * p.C, gl, p.C, v);
-            if (p.x) load_row<T, W, G>(static_cast<const T *>(p.x) + r * p.C, gl, p.C, x);
-            if (p.gate) {
-                const int64_t gr = (uint32_t)r / p.rpg;
-                if (gr != held) {
-                    load_gate<T, W, G>(p, gr, gl, a);
-                    held = gr;
-#pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        float slope;
-                        activate(p.act, a[j], a[j], slope);
-                    }
+                for (int j = 0; j < E; ++j) {
+                    float slope;
+                    activate(p.act, a[j], a[j], slope);
                 }
             }
         }
+        fetch(r + (int64_t)gridDim.x * GR);
         if (p.post != EVFLY_NORM_NONE) {
             normalise<W, G>(v, p.post, gl, p.C, p.inv_c, p.eps, red, turn);
 #pragma unroll
@@ -282,19 +298,26 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
 #pragma unroll
         for (int j = 0; j < E; ++j) a[j] = slope[j] = 1.f;
         if (p.gate && p.rpg > 1) load_act(lo / p.rpg);
+        Row<T, W, G> nf, nx, ny, nh;
+        nf.clear(); nx.clear(); ny.clear(); nh.clear();
+        auto fetch = [&](int64_t r) {
+            if (r >= hi) return;
+            nf.fetch(static_cast<const T *>(p.f) + r * p.C, gl, p.C);
+            if (p.x) nx.fetch(static_cast<const T *>(p.x) + r * p.C, gl, p.C);
+            if (p.dy) ny.fetch(static_cast<const T *>(p.dy) + r * p.C, gl, p.C);
+            if (p.dh) nh.fetch(static_cast<const T *>(p.dh) + r * p.C, gl, p.C);
+        };
+        fetch(lo + gi);
         for (int64_t r0 = lo; r0 < hi; r0 += GR) {
             const int64_t r = r0 + gi;
             const bool live = r < hi;
             float f[E], x[E], dy[E], dh[E];
-#pragma unroll
-            for (int j = 0; j < E; ++j) f[j] = x[j] = dy[j] = dh[j] = 0.f;
-            if (live) {
-                load_row<T, W, G>(static_cast<const T *>(p.f) + r * p.C, gl, p.C, f);
-                if (p.x) load_row<T, W, G>(static_cast<const T *>(p.x) + r * p.C, gl, p.C, x);
-                if (p.dy) load_row<T, W, G>(static_cast<const T *>(p.dy) + r * p.C, gl, p.C, dy);
-                if (p.dh) load_row<T, W, G>(static_cast<const T *>(p.dh) + r * p.C, gl, p.C, dh);
-                if (p.gate && p.rpg == 1) load_act(r);
-            }
+            nf.widen(f);
+            nx.widen(x);
+            ny.widen(dy);
+            nh.widen(dh);
+            if (live && p.gate && p.rpg == 1) load_act(r);
+            fetch(r + GR);
             // forward again: fh = normalised f, u = its affine form
             float r1 = 1.f, u[E];
             if (p.post != EVFLY_NORM_NONE) r1 = normalise<W, G>(f, p.post, gl, p.C, p.inv_c, p.eps, red, turn);
