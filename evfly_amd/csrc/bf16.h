@@ -66,4 +66,29 @@ template <> struct Elem<bf16_t> {
     __device__ static __forceinline__ void st1(bf16_t *p, float v) { *p = f2bf_dev(v); }
 };
 
+// 16 and 8 bytes at any element's address: gfx950 loads and stores them whole without alignment (a row of an odd width costs the cache lines it
+// straddles, not a load per element)
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ uint4 load16_any(const void *p) {
+    const u32x4_any t = *reinterpret_cast<const u32x4_any *>(p);
+    return make_uint4(t.x, t.y, t.z, t.w);
+}
+__device__ __forceinline__ void store16_any(void *p, uint4 v) { *reinterpret_cast<u32x4_any *>(p) = u32x4_any{v.x, v.y, v.z, v.w}; }
+__device__ __forceinline__ void store8_any(void *p, uint2 v) { *reinterpret_cast<u32x2_any *>(p) = u32x2_any{v.x, v.y}; }
+
+// the 16-byte piece of a row of which `n` values are left: whole, its first n values and zeros, or nothing (n <= 0)
+template <typename T> __device__ __forceinline__ uint4 load_piece(const T *at, int n) {
+    constexpr int V = 16 / sizeof(T);
+    if (n >= V) return load16_any(at);
+    union { T v[V]; uint4 u; } r;
+    r.u = make_uint4(0, 0, 0, 0);
+    if (n > 0) {
+#pragma unroll
+        for (int e = 0; e < V - 1; ++e)
+            if (e < n) r.v[e] = at[e];
+    }
+    return r.u;
+}
+
 }  // namespace evfly

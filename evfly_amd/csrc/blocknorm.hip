@@ -1,15 +1,14 @@
 // Block norm: y = res_scale x + act(gate) norm_post(f), h = norm_pre(y), and its gradients. Bound by HBM: forward reads x, f (gate) and writes y, h once;
 // backward reads x, f (gate), dy, dh, forms the forward's row again in registers and writes dx, df (d_gate) once, beside the column sums.
 //
-// A row is held by a group of G lanes in registers from its load to its stores, eight values per lane (one 16-byte vector of bf16, two of fp32, or
-// eight single elements where the rows are not 16-byte aligned), so G is the smallest power of two that covers the channels: rows of up to 512
+// A row is held by a group of G lanes in registers from its load to its stores, eight values per lane (one 16-byte piece of bf16, two of fp32, at
+// any alignment), so G is the smallest power of two that covers the channels: rows of up to 512
 // channels share waves, longer ones take a block of up to 1024 threads. Each group keeps its columns of every weight vector in registers over all the rows it
 // visits. Mean and variance are two passes over the registers, fp32.
 //
 // Column sums (weights, biases, residual scale, a broadcast gate) are kept per lane over the block's rows, added over the block's groups in LDS, written
 // as one partial row per block and added in block order by k_bn_columns: no atomics, the same bits on every call.
 #include <cmath>
-#include <type_traits>
 
 #include "bf16.h"
 #include "common.h"
@@ -38,67 +37,72 @@ struct BnArgs {
 };
 enum { K_ALPHA, K_W1, K_B1, K_W2, K_B2, K_GATE, K_N };
 
-// A lane's eight values are E / W pieces of W neighbouring ones: value j lies in column ((j / W) G + gl) W + j % W. Columns behind C read as zero. A row is
-// fetched as it lies in memory (one row ahead of its use) and widened when its turn comes.
-template <typename S, int W, int G> struct Row {
-    static constexpr int VS = W == 1 ? 1 : 16 / sizeof(S);               // values per load
-    typename std::conditional<W == 1, S, uint4>::type raw[E / VS];
-    __device__ __forceinline__ void fetch(const S *row, int gl, int C) {
+// A lane's eight values are 16-byte pieces of VS neighbouring ones: value j lies in column ((j / VS) G + gl) VS + j % VS. Columns behind C read as zero. A
+// row is fetched as it lies in memory (one row ahead of its use) and widened when its turn comes.
+template <typename T> constexpr int VS = 16 / sizeof(T);
+template <typename T, int G> __device__ __forceinline__ int column(int gl, int j) { return (j / VS<T> * G + gl) * VS<T> + j % VS<T>; }
+
+template <typename T, int G> struct Row {
+    uint4 raw[E / VS<T>];
+    __device__ __forceinline__ void fetch(const T *row, int gl, int C) {
 #pragma unroll
-        for (int k = 0; k < E / VS; ++k) {
-            const int c = (k * VS / W * G + gl) * W + k * VS % W;
-            if constexpr (W == 1) raw[k] = c < C ? row[c] : S(0);
-            else raw[k] = c < C ? *reinterpret_cast<const uint4 *>(row + c) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < E / VS<T>; ++k) {
+            const int c = (k * G + gl) * VS<T>;
+            raw[k] = load_piece<T>(row + c, C - c);
         }
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int k = 0; k < E / VS; ++k) raw[k] = {};
+        for (int k = 0; k < E / VS<T>; ++k) raw[k] = make_uint4(0, 0, 0, 0);
     }
     __device__ __forceinline__ void widen(float (&v)[E]) const {
 #pragma unroll
-        for (int k = 0; k < E / VS; ++k) {
-            float t[VS];
-            if constexpr (W == 1) t[0] = Elem<S>::ld1(&raw[k]);
-            else Elem<S>::load(reinterpret_cast<const S *>(&raw[k]), t);
+        for (int k = 0; k < E / VS<T>; ++k) {
+            float t[VS<T>];
+            Elem<T>::load(reinterpret_cast<const T *>(&raw[k]), t);
 #pragma unroll
-            for (int i = 0; i < VS; ++i) v[k * VS + i] = t[i];
+            for (int i = 0; i < VS<T>; ++i) v[k * VS<T> + i] = t[i];
         }
     }
 };
-template <typename S, int W, int G> __device__ __forceinline__ void store_row(S *row, int gl, int C, const float (&v)[E]) {
-    constexpr int VS = 16 / sizeof(S);
+template <typename T, int G> __device__ __forceinline__ void store_row(T *row, int gl, int C, const float (&v)[E]) {
 #pragma unroll
-    for (int j = 0; j < E / W; ++j) {
-        const int c = (j * G + gl) * W;
-        if (c < C) {
-            if constexpr (W == 1) Elem<S>::st1(row + c, v[j]);
-            else
+    for (int k = 0; k < E / VS<T>; ++k) {
+        const int c = (k * G + gl) * VS<T>;
+        float t[VS<T>];
 #pragma unroll
-                for (int e = 0; e < W; e += VS) {
-                    float t[VS];
+        for (int i = 0; i < VS<T>; ++i) t[i] = v[k * VS<T> + i];
+        if (c + VS<T> <= C) {
+            uint4 u;
+            Elem<T>::store(reinterpret_cast<T *>(&u), t);
+            store16_any(row + c, u);
+        } else if (c < C) {
 #pragma unroll
-                    for (int i = 0; i < VS; ++i) t[i] = v[j * W + e + i];
-                    Elem<S>::store(row + c + e, t);
-                }
+            for (int i = 0; i < VS<T> - 1; ++i)
+                if (c + i < C) Elem<T>::st1(row + c + i, t[i]);
         }
     }
 }
-// fp32 vectors whose base may be unaligned (parameters): W neighbouring values, single loads
-template <int W, int G> __device__ __forceinline__ void load_vec(const float *p, int gl, int C, float other, float (&v)[E]) {
+// the same columns of an fp32 vector (`other` where there is none, and behind C)
+template <typename T, int G> __device__ __forceinline__ void load_vec(const float *p, int gl, int C, float other, float (&v)[E]) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const int c = ((j / W) * G + gl) * W + j % W;
-        v[j] = p && c < C ? p[c] : other;
+    for (int j = 0; j < E; j += 4) {
+        const int c = column<T, G>(gl, j);
+        if (p && c + 4 <= C) {
+            const uint4 u = load16_any(p + c);
+            v[j] = __uint_as_float(u.x); v[j + 1] = __uint_as_float(u.y); v[j + 2] = __uint_as_float(u.z); v[j + 3] = __uint_as_float(u.w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j + i] = p && c + i < C ? p[c + i] : other;
+        }
     }
 }
 // a gate row in its own type (the tokens' or fp32)
-template <typename T, int W, int G> __device__ __forceinline__ void load_gate(const BnArgs &p, int64_t row, int gl, float (&v)[E]) {
+template <typename T, int G> __device__ __forceinline__ void load_gate(const BnArgs &p, int64_t row, int gl, float (&v)[E]) {
     if (p.gate_f32) {
-        const float *g = static_cast<const float *>(p.gate) + row * p.C;
-        load_vec<W, G>(g, gl, p.C, 0.f, v);
+        load_vec<T, G>(static_cast<const float *>(p.gate) + row * p.C, gl, p.C, 0.f, v);
     } else {
-        Row<T, W, G> t;
+        Row<T, G> t;
         t.fetch(static_cast<const T *>(p.gate) + row * p.C, gl, p.C);
         t.widen(v);
     }
@@ -151,7 +155,7 @@ template <int G, int N> __device__ __forceinline__ void row_sum(float (&v)[N], f
     }
 }
 // v -> (v - mean) / sqrt(var + eps) in place (EVFLY_NORM_RMS: mean = 0); columns behind C stay zero. Returns 1 / sqrt(..).
-template <int W, int G> __device__ __forceinline__ float normalise(float (&v)[E], int kind, int gl, int C, float inv_c, float eps, float *red, int &turn) {
+template <typename T, int G> __device__ __forceinline__ float normalise(float (&v)[E], int kind, int gl, int C, float inv_c, float eps, float *red, int &turn) {
     float mu = 0.f;
     if (kind == EVFLY_NORM_LAYER) {
         float s[1] = {0.f};
@@ -163,7 +167,7 @@ template <int W, int G> __device__ __forceinline__ float normalise(float (&v)[E]
     float q[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-        const int c = ((j / W) * G + gl) * W + j % W;
+        const int c = column<T, G>(gl, j);
         v[j] = c < C ? v[j] - mu : 0.f;
         q[0] = fmaf(v[j], v[j], q[0]);
     }
@@ -174,20 +178,20 @@ template <int W, int G> __device__ __forceinline__ float normalise(float (&v)[E]
     return r;
 }
 
-template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void k_bn_fwd(BnArgs p) {
+template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void k_bn_fwd(BnArgs p) {
     constexpr int NT = G > 256 ? G : 256, GR = NT / G;
     __shared__ float red[64];
     int turn = 0;
     const int gl = threadIdx.x % G, gi = threadIdx.x / G;
     float w1[E], b1[E], w2[E], b2[E], al[E], a[E];
-    load_vec<W, G>(p.w1, gl, p.C, 1.f, w1);
-    load_vec<W, G>(p.b1, gl, p.C, 0.f, b1);
-    load_vec<W, G>(p.w2, gl, p.C, 1.f, w2);
-    load_vec<W, G>(p.b2, gl, p.C, 0.f, b2);
-    load_vec<W, G>(p.alpha, gl, p.C, 1.f, al);
+    load_vec<T, G>(p.w1, gl, p.C, 1.f, w1);
+    load_vec<T, G>(p.b1, gl, p.C, 0.f, b1);
+    load_vec<T, G>(p.w2, gl, p.C, 1.f, w2);
+    load_vec<T, G>(p.b2, gl, p.C, 0.f, b2);
+    load_vec<T, G>(p.alpha, gl, p.C, 1.f, al);
     int64_t held = -1;                               // gate row in a[]
     const bool token_gate = p.gate && p.rpg == 1 && !p.gate_f32;
-    Row<T, W, G> nf, nx, ng;
+    Row<T, G> nf, nx, ng;
     nf.clear(); nx.clear(); ng.clear();
     auto fetch = [&](int64_t r) {
         if (r >= p.rows) return;
@@ -206,7 +210,7 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
             const int64_t gr = p.rpg == 1 ? r : (uint32_t)r / p.rpg;
             if (gr != held) {
                 if (token_gate) ng.widen(a);
-                else load_gate<T, W, G>(p, gr, gl, a);
+                else load_gate<T, G>(p, gr, gl, a);
                 held = gr;
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
@@ -217,7 +221,7 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
         }
         fetch(r + (int64_t)gridDim.x * GR);
         if (p.post != EVFLY_NORM_NONE) {
-            normalise<W, G>(v, p.post, gl, p.C, p.inv_c, p.eps, red, turn);
+            normalise<T, G>(v, p.post, gl, p.C, p.inv_c, p.eps, red, turn);
 #pragma unroll
             for (int j = 0; j < E; ++j) v[j] = fmaf(v[j], w1[j], b1[j]);
         }
@@ -227,18 +231,18 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
         if (p.x)
 #pragma unroll
             for (int j = 0; j < E; ++j) v[j] = fmaf(al[j], x[j], v[j]);
-        if (live && p.y) store_row<T, W, G>(static_cast<T *>(p.y) + r * p.C, gl, p.C, v);
+        if (live && p.y) store_row<T, G>(static_cast<T *>(p.y) + r * p.C, gl, p.C, v);
         if (p.pre != EVFLY_NORM_NONE) {
-            normalise<W, G>(v, p.pre, gl, p.C, p.inv_c, p.eps, red, turn);
+            normalise<T, G>(v, p.pre, gl, p.C, p.inv_c, p.eps, red, turn);
 #pragma unroll
             for (int j = 0; j < E; ++j) v[j] = fmaf(v[j], w2[j], b2[j]);
-            if (live) store_row<T, W, G>(static_cast<T *>(p.h) + r * p.C, gl, p.C, v);
+            if (live) store_row<T, G>(static_cast<T *>(p.h) + r * p.C, gl, p.C, v);
         }
     }
 }
 
 // Sum of one value array over the block's groups; group 0's lanes hold the result (after the wave exchange: lanes < G of wave 0 for G <= 64).
-template <int W, int G, int NT> __device__ __forceinline__ void block_columns(float (&v)[E], float *lds, int gl, int gi) {
+template <int G, int NT> __device__ __forceinline__ void block_columns(float (&v)[E], float *lds, int gl, int gi) {
     if constexpr (G < 64)
 #pragma unroll
         for (int d = G; d < 64; d *= 2)
@@ -261,25 +265,29 @@ template <int W, int G, int NT> __device__ __forceinline__ void block_columns(fl
             }
     }
 }
-template <int W, int G> __device__ __forceinline__ void store_columns(float *out, int gl, int C, const float (&v)[E]) {
+template <typename T, int G> __device__ __forceinline__ void store_columns(float *out, int gl, int C, const float (&v)[E]) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const int c = ((j / W) * G + gl) * W + j % W;
-        if (c < C) out[c] = v[j];
+    for (int j = 0; j < E; j += 4) {
+        const int c = column<T, G>(gl, j);
+        if (c + 4 <= C) store16_any(out + c, make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])));
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < C) out[c + i] = v[j + i];
     }
 }
 
-template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void k_bn_bwd(BnArgs p) {
+template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void k_bn_bwd(BnArgs p) {
     constexpr int NT = G > 256 ? G : 256, GR = NT / G, GW = G < 64 ? 64 : G;
     __shared__ float red[64];
     __shared__ float lds[NT / GW > 1 ? NT / GW * E * G : 1];
     int turn = 0;
     const int gl = threadIdx.x % G, gi = threadIdx.x / G;
     float w1[E], b1[E], w2[E], al[E];
-    load_vec<W, G>(p.w1, gl, p.C, 1.f, w1);
-    load_vec<W, G>(p.b1, gl, p.C, 0.f, b1);
-    load_vec<W, G>(p.w2, gl, p.C, 1.f, w2);
-    load_vec<W, G>(p.alpha, gl, p.C, 1.f, al);
+    load_vec<T, G>(p.w1, gl, p.C, 1.f, w1);
+    load_vec<T, G>(p.b1, gl, p.C, 0.f, b1);
+    load_vec<T, G>(p.w2, gl, p.C, 1.f, w2);
+    load_vec<T, G>(p.alpha, gl, p.C, 1.f, al);
     float sa[E], sw1[E], sb1[E], sw2[E], sb2[E], sg[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) sa[j] = sw1[j] = sb1[j] = sw2[j] = sb2[j] = sg[j] = 0.f;
@@ -291,14 +299,14 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
         const int64_t hi = min(lo + (int64_t)p.unit_rows, base + (int64_t)p.span);
         float a[E], slope[E];
         auto load_act = [&](int64_t row) {
-            load_gate<T, W, G>(p, row, gl, a);
+            load_gate<T, G>(p, row, gl, a);
 #pragma unroll
             for (int j = 0; j < E; ++j) activate(p.act, a[j], a[j], slope[j]);
         };
 #pragma unroll
         for (int j = 0; j < E; ++j) a[j] = slope[j] = 1.f;
         if (p.gate && p.rpg > 1) load_act(lo / p.rpg);
-        Row<T, W, G> nf, nx, ny, nh;
+        Row<T, G> nf, nx, ny, nh;
         nf.clear(); nx.clear(); ny.clear(); nh.clear();
         auto fetch = [&](int64_t r) {
             if (r >= hi) return;
@@ -320,7 +328,7 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
             fetch(r + GR);
             // forward again: fh = normalised f, u = its affine form
             float r1 = 1.f, u[E];
-            if (p.post != EVFLY_NORM_NONE) r1 = normalise<W, G>(f, p.post, gl, p.C, p.inv_c, p.eps, red, turn);
+            if (p.post != EVFLY_NORM_NONE) r1 = normalise<T, G>(f, p.post, gl, p.C, p.inv_c, p.eps, red, turn);
 #pragma unroll
             for (int j = 0; j < E; ++j) u[j] = p.post != EVFLY_NORM_NONE ? fmaf(f[j], w1[j], b1[j]) : f[j];
             if (p.pre != EVFLY_NORM_NONE) {
@@ -330,7 +338,7 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
                     y[j] = a[j] * u[j];
                     if (p.x) y[j] = fmaf(al[j], x[j], y[j]);
                 }
-                const float r2 = normalise<W, G>(y, p.pre, gl, p.C, p.inv_c, p.eps, red, turn);
+                const float r2 = normalise<T, G>(y, p.pre, gl, p.C, p.inv_c, p.eps, red, turn);
                 float s[2] = {0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
@@ -355,7 +363,7 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
                     if (live) sa[j] = fmaf(dy[j], x[j], sa[j]);
                     t[j] = al[j] * dy[j];
                 }
-                if (live && p.dx) store_row<T, W, G>(static_cast<T *>(p.dx) + r * p.C, gl, p.C, t);
+                if (live && p.dx) store_row<T, G>(static_cast<T *>(p.dx) + r * p.C, gl, p.C, t);
             }
             if (p.gate) {
 #pragma unroll
@@ -365,8 +373,8 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
                     dy[j] *= a[j];
                 }
                 if (live && p.dgate && p.rpg == 1) {
-                    if (p.gate_f32) store_columns<W, G>(static_cast<float *>(p.dgate) + r * p.C, gl, p.C, t);
-                    else store_row<T, W, G>(static_cast<T *>(p.dgate) + r * p.C, gl, p.C, t);
+                    if (p.gate_f32) store_columns<T, G>(static_cast<float *>(p.dgate) + r * p.C, gl, p.C, t);
+                    else store_row<T, G>(static_cast<T *>(p.dgate) + r * p.C, gl, p.C, t);
                 }
             }
             if (p.post != EVFLY_NORM_NONE) {
@@ -378,7 +386,7 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
                         sw1[j] = fmaf(dy[j], f[j], sw1[j]);
                     }
                     dy[j] *= w1[j];
-                    const float in = ((j / W) * G + gl) * W + j % W < p.C ? dy[j] : 0.f;
+                    const float in = column<T, G>(gl, j) < p.C ? dy[j] : 0.f;
                     s[0] += in;
                     s[1] = fmaf(in, f[j], s[1]);
                 }
@@ -387,14 +395,14 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
 #pragma unroll
                 for (int j = 0; j < E; ++j) dy[j] = r1 * (dy[j] - m0 - f[j] * m1);
             }
-            if (live) store_row<T, W, G>(static_cast<T *>(p.df) + r * p.C, gl, p.C, dy);
+            if (live) store_row<T, G>(static_cast<T *>(p.df) + r * p.C, gl, p.C, dy);
         }
         if (gate_rows) {
-            block_columns<W, G, NT>(sg, lds, gl, gi);
+            block_columns<G, NT>(sg, lds, gl, gi);
             if (gi == 0) {
-                if (p.parts > 1) store_columns<W, G>(p.gate_part + (int64_t)unit * p.C, gl, p.C, sg);
-                else if (p.gate_f32) store_columns<W, G>(static_cast<float *>(p.dgate) + (int64_t)grow * p.C, gl, p.C, sg);
-                else store_row<T, W, G>(static_cast<T *>(p.dgate) + (int64_t)grow * p.C, gl, p.C, sg);
+                if (p.parts > 1) store_columns<T, G>(p.gate_part + (int64_t)unit * p.C, gl, p.C, sg);
+                else if (p.gate_f32) store_columns<T, G>(static_cast<float *>(p.dgate) + (int64_t)grow * p.C, gl, p.C, sg);
+                else store_row<T, G>(static_cast<T *>(p.dgate) + (int64_t)grow * p.C, gl, p.C, sg);
             }
 #pragma unroll
             for (int j = 0; j < E; ++j) sg[j] = 0.f;
@@ -403,8 +411,8 @@ template <typename T, int W, int G> __global__ __launch_bounds__(G > 256 ? G : 2
     float *const out = p.cols + (int64_t)blockIdx.x * K_N * p.C;
     auto flush = [&](int kind, float (&v)[E]) {
         if (!(p.want >> kind & 1)) return;
-        block_columns<W, G, NT>(v, lds, gl, gi);
-        if (gi == 0) store_columns<W, G>(out + kind * p.C, gl, p.C, v);
+        block_columns<G, NT>(v, lds, gl, gi);
+        if (gi == 0) store_columns<T, G>(out + kind * p.C, gl, p.C, v);
     };
     flush(K_ALPHA, sa); flush(K_W1, sw1); flush(K_B1, sb1); flush(K_W2, sw2); flush(K_B2, sb2); flush(K_GATE, sg);
 }
@@ -441,29 +449,28 @@ __global__ __launch_bounds__(1024) void k_bn_columns(BnSums p) {
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename T, int W, int G> int bn_launch(const BnArgs &p, bool backward, unsigned blocks, hipStream_t st) {
+template <typename T, int G> int bn_launch(const BnArgs &p, bool backward, unsigned blocks, hipStream_t st) {
     constexpr int NT = G > 256 ? G : 256;
-    if (backward) hipLaunchKernelGGL((k_bn_bwd<T, W, G>), dim3(blocks), dim3(NT), 0, st, p);
-    else hipLaunchKernelGGL((k_bn_fwd<T, W, G>), dim3(blocks), dim3(NT), 0, st, p);
+    if (backward) hipLaunchKernelGGL((k_bn_bwd<T, G>), dim3(blocks), dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((k_bn_fwd<T, G>), dim3(blocks), dim3(NT), 0, st, p);
     EVFLY_LAUNCH_CHECK();
     return 0;
 }
-template <typename T, int W> int bn_group(const BnArgs &p, int G, bool backward, unsigned blocks, hipStream_t st) {
+template <typename T> int bn_group(const BnArgs &p, int G, bool backward, unsigned blocks, hipStream_t st) {
     switch (G) {
-    case 4: return bn_launch<T, W, 4>(p, backward, blocks, st);
-    case 8: return bn_launch<T, W, 8>(p, backward, blocks, st);
-    case 16: return bn_launch<T, W, 16>(p, backward, blocks, st);
-    case 32: return bn_launch<T, W, 32>(p, backward, blocks, st);
-    case 64: return bn_launch<T, W, 64>(p, backward, blocks, st);
-    case 128: return bn_launch<T, W, 128>(p, backward, blocks, st);
-    case 256: return bn_launch<T, W, 256>(p, backward, blocks, st);
-    case 512: return bn_launch<T, W, 512>(p, backward, blocks, st);
-    default: return bn_launch<T, W, 1024>(p, backward, blocks, st);
+    case 4: return bn_launch<T, 4>(p, backward, blocks, st);
+    case 8: return bn_launch<T, 8>(p, backward, blocks, st);
+    case 16: return bn_launch<T, 16>(p, backward, blocks, st);
+    case 32: return bn_launch<T, 32>(p, backward, blocks, st);
+    case 64: return bn_launch<T, 64>(p, backward, blocks, st);
+    case 128: return bn_launch<T, 128>(p, backward, blocks, st);
+    case 256: return bn_launch<T, 256>(p, backward, blocks, st);
+    case 512: return bn_launch<T, 512>(p, backward, blocks, st);
+    default: return bn_launch<T, 1024>(p, backward, blocks, st);
     }
 }
-int bn_run(const BnArgs &p, int dtype, bool vec, int G, bool backward, unsigned blocks, hipStream_t st) {
-    if (dtype == EVFLY_DTYPE_F32) return vec ? bn_group<float, 4>(p, G, backward, blocks, st) : bn_group<float, 1>(p, G, backward, blocks, st);
-    return vec ? bn_group<bf16_t, 8>(p, G, backward, blocks, st) : bn_group<bf16_t, 1>(p, G, backward, blocks, st);
+int bn_run(const BnArgs &p, int dtype, int G, bool backward, unsigned blocks, hipStream_t st) {
+    return dtype == EVFLY_DTYPE_F32 ? bn_group<float>(p, G, backward, blocks, st) : bn_group<bf16_t>(p, G, backward, blocks, st);
 }
 
 int lanes_for(int C) {
@@ -534,11 +541,9 @@ extern "C" int evfly_block_norm_forward(const void *f, const void *x, const void
     p.f = f; p.x = x; p.gate = gate; p.alpha = res_scale; p.w1 = post_weight; p.b1 = post_bias; p.w2 = pre_weight; p.b2 = pre_bias;
     p.y = y; p.h = h; p.post = post_kind; p.pre = pre_kind; p.act = gate_act; p.gate_f32 = gate_f32; p.C = channels;
     p.rows = (uint32_t)rows; p.rpg = gate ? (uint32_t)rows_per_gate : 1u; p.eps = eps; p.inv_c = 1.f / (float)channels;
-    const int V = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
-    const bool vec = channels % V == 0 && aligned16(f) && aligned16(x) && aligned16(y) && aligned16(h) && (gate_f32 || aligned16(gate));
     const int G = lanes_for(channels), GR = (G > 256 ? G : 256) / G;
     const int64_t need = (rows + GR - 1) / GR, most = 8 * kNumCU;
-    return bn_run(p, dtype, vec, G, false, (unsigned)(need < most ? need : most), as_stream(stream));
+    return bn_run(p, dtype, G, false, (unsigned)(need < most ? need : most), as_stream(stream));
 }
 
 extern "C" int64_t evfly_block_norm_workspace_bytes(int64_t rows, int channels, int64_t rows_per_gate, int dtype) {
@@ -571,9 +576,6 @@ extern "C" int evfly_block_norm_backward(const void *f, const void *x, const voi
     const bool streams = rpg > 1 && rpg < rows;
     p.unit_rows = b.unit_rows; p.parts = b.parts; p.units = b.units; p.span = (uint32_t)(streams ? rpg : rows);
     float *const vecs[K_N] = {d_res_scale, d_post_weight, d_post_bias, d_pre_weight, d_pre_bias, nullptr};
-    const int V = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
-    const bool vec = channels % V == 0 && aligned16(f) && aligned16(x) && aligned16(dy) && aligned16(dh) && aligned16(df) && aligned16(dx) &&
-                     (gate_f32 || (aligned16(gate) && aligned16(d_gate)));
     BnSums s{};
     s.n = (int)b.blocks; s.C = channels; s.row_stride = (int64_t)K_N * channels;
     int m = 0;
@@ -588,7 +590,7 @@ extern "C" int evfly_block_norm_backward(const void *f, const void *x, const voi
         ++m;
     }
     if (rows > 0)
-        if (int rc = bn_run(p, dtype, vec, b.G, true, b.blocks, st)) return rc;
+        if (int rc = bn_run(p, dtype, b.G, true, b.blocks, st)) return rc;
     if (m) hipLaunchKernelGGL(k_bn_columns, dim3((channels + 63) / 64, m, 1), dim3(1024), 0, st, s);
     if (streams && d_gate && b.parts > 1) {
         BnSums g{};

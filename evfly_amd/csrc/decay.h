@@ -39,8 +39,8 @@ struct DecaySplit { int nseg, seg_len; };
 DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype, bool backward);
 
 // All passes have the same da and dc classes. STATE: the segments' own states only (into slot segment + 1 of seg), no output.
-int decay_passes_f32(const DecayPasses &p, bool state, bool vec, hipStream_t st);
-int decay_passes_bf16(const DecayPasses &p, bool state, bool vec, hipStream_t st);
+int decay_passes_f32(const DecayPasses &p, bool state, hipStream_t st);
+int decay_passes_bf16(const DecayPasses &p, bool state, hipStream_t st);
 
 inline int decay_tile_a(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }      // the a dimension whole (its rows are summed in registers)
 inline int decay_tile_c(int d) { return d <= 32 ? 32 : 64; }                       // columns of c per block

@@ -173,14 +173,9 @@ struct Tokens {              // one token tensor: pointer, element strides, head
     int64_t s[3];
     int r, d;
 };
-bool vec_ok(const Tokens &t, int vec) {
-    return aligned16(t.p) && t.d % vec == 0 && t.s[0] % vec == 0 && t.s[1] % vec == 0 && t.s[2] % vec == 0;
-}
-
 // One call's passes: roles filled in, tiles chosen, launched together where the tiles agree.
 struct Run {
     int dtype;
-    bool vec = true;                       // every tensor of the call in 16-byte pieces
     hipStream_t st;
     DecayPass base;                        // what all passes share
 
@@ -193,7 +188,7 @@ struct Run {
         return p;
     }
     int launch(const DecayPasses &ps, bool state) const {
-        return dtype == EVFLY_DTYPE_F32 ? decay_passes_f32(ps, state, vec, st) : decay_passes_bf16(ps, state, vec, st);
+        return dtype == EVFLY_DTYPE_F32 ? decay_passes_f32(ps, state, st) : decay_passes_bf16(ps, state, st);
     }
     // slots of up to two state sequences [dk][dv], each from its own state pass
     int segment_states(const DecayPass *own, int np, int dk, int dv) const {
@@ -314,8 +309,7 @@ extern "C" int evfly_decay_attention_forward(const void *q, const void *k, const
         a.T = tokens; a.H = heads; a.rep = rep; a.dk = dk; a.dv = dv; a.scale = scale;
         return dtype == EVFLY_DTYPE_F32 ? step_all<float>(a, n_streams, st) : step_all<bf16_t>(a, n_streams, st);
     }
-    const int vec = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
-    Run run{dtype, vec_ok(tq, vec) && vec_ok(tk, vec) && vec_ok(tv, vec) && aligned16(out), st, DecayPass{}};
+    Run run{dtype, st, DecayPass{}};
     const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype, false);
     DecayPass &b = run.base;
     b.log_decay = log_decay; b.lengths = lengths; b.n = n_streams; b.T = tokens; b.H = heads; b.nseg = sp.nseg; b.seg_len = sp.seg_len;
@@ -348,8 +342,7 @@ extern "C" int evfly_decay_attention_backward(const void *q, const void *k, cons
     token_strides(strides_host ? strides_host + 6 : nullptr, tokens, kv_heads, dv, tv.s);
     token_strides(nullptr, tokens, heads, dv, to.s);
     EVFLY_REQUIRE(!d_state_in || d_state_in != d_state_out, "decay_attention_backward: d_state_in is d_state_out");
-    const int vec = dtype == EVFLY_DTYPE_F32 ? 4 : 8;
-    Run run{dtype, vec_ok(tq, vec) && vec_ok(tk, vec) && vec_ok(tv, vec) && vec_ok(to, vec) && aligned16(dq) && aligned16(dk_out) && aligned16(dv_out), st, DecayPass{}};
+    Run run{dtype, st, DecayPass{}};
     const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype, true);
     char *const w = static_cast<char *>(workspace);
     float *const seg = reinterpret_cast<float *>(w), *const part_k = reinterpret_cast<float *>(w + ws.part_k), *const part_v = reinterpret_cast<float *>(w + ws.part_v);

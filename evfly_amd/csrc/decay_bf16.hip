@@ -4,5 +4,5 @@
 #include "decay_kernel.h"
 
 namespace evfly {
-int decay_passes_bf16(const DecayPasses &p, bool state, bool vec, hipStream_t st) { return decay::launch_all<bf16_t>(p, state, vec, st); }
+int decay_passes_bf16(const DecayPasses &p, bool state, hipStream_t st) { return decay::launch_all<bf16_t>(p, state, st); }
 }  // namespace evfly

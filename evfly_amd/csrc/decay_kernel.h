@@ -121,16 +121,6 @@ template <> struct Mm<bf16_t> {
     }
 };
 
-// 16 bytes of a token row of which `n` values are left (n <= 0: none), zeros behind them. VEC: rows are 16-byte aligned and end with a whole piece.
-template <typename T, bool VEC> __device__ __forceinline__ uint4 load16(const T *at, int n) {
-    constexpr int V = 16 / sizeof(T);
-    if (VEC) return n > 0 ? *reinterpret_cast<const uint4 *>(at) : make_uint4(0, 0, 0, 0);
-    union { T v[V]; uint4 u; } r;
-#pragma unroll
-    for (int e = 0; e < V; ++e) r.v[e] = e < n ? at[e] : T(0);
-    return r.u;
-}
-
 template <typename T, int DA, int DC> struct Lds {
     static constexpr int RB = DA * (int)sizeof(T) + 16;        // row strides in bytes: 16 more than the row, so that 16 rows read at one column
     static constexpr int RC = DC * (int)sizeof(T) + 16;        // spread over the banks
@@ -148,7 +138,7 @@ template <typename T, int DA, int DC, bool STATE> constexpr int blocks_per_cu() 
 }
 
 // STATE: the segment's own state only (no output), for the sequences that are split into segments.
-template <typename T, int DA, int DC, bool VEC, bool STATE>
+template <typename T, int DA, int DC, bool STATE>
 __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_decay_chunk(DecayPasses ps) {
     typedef Mm<T> M;
     typedef typename M::frag frag;
@@ -230,19 +220,19 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
 #pragma unroll
         for (int x = 0; x < NB; ++x, bq += bstep) {
             rb[x] = make_uint4(0, 0, 0, 0);
-            if (br + x * RPB < left) rb[x] = load16<T, VEC>(bq, p.da - bcol);
+            if (br + x * RPB < left) rb[x] = load_piece<T>(bq, p.da - bcol);
         }
 #pragma unroll
         for (int x = 0; x < NV; ++x, cq += cstep) {
             rc[x] = make_uint4(0, 0, 0, 0);
-            if (cr + x * RPC < left) rc[x] = load16<T, VEC>(cq, dcw - ccol);
+            if (cr + x * RPC < left) rc[x] = load_piece<T>(cq, dcw - ccol);
         }
         if (!STATE) {
 #pragma unroll
             for (int k = 0; k < KA; ++k) {
                 union { uint4 u4; frag f; } t;
                 t.u4 = make_uint4(0, 0, 0, 0);
-                if (ar < left) t.u4 = load16<T, VEC>(aq + k * M::KB, p.da - k * M::KB - g * V);
+                if (ar < left) t.u4 = load_piece<T>(aq + k * M::KB, p.da - k * M::KB - g * V);
                 fa_next[k] = t.f;
             }
             aq += astep;
@@ -326,33 +316,25 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
                 }
                 const int c = 16 * y + 4 * g;
                 if (there && c < dcw) {
-                    if (p.out_f32) {
+                    const uint4 w4 = make_uint4(__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3]));
+                    if (sizeof(T) == 4 || p.out_f32) {
                         float *d = static_cast<float *>(p.out) + oi + c;
-                        if (VEC) *reinterpret_cast<f32x4 *>(d) = acc;
+                        if (c + 4 <= dcw) store16_any(d, w4);
                         else
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
+                            for (int e = 0; e < 3; ++e)
                                 if (c + e < dcw) d[e] = acc[e];
                     } else {
                         T *d = static_cast<T *>(p.out) + oi + c;
-                        if (sizeof(T) == 4) {
-                            if (VEC) *reinterpret_cast<f32x4 *>(d) = acc;
-                            else
+                        if (c + 4 <= dcw) store8_any(d, make_uint2(pack_bf2(acc[0], acc[1]), pack_bf2(acc[2], acc[3])));
+                        else
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (c + e < dcw) Elem<T>::st1(d + e, acc[e]);
-                        } else {
-                            if (VEC) *reinterpret_cast<uint2 *>(d) = make_uint2(pack_bf2(acc[0], acc[1]), pack_bf2(acc[2], acc[3]));
-                            else
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (c + e < dcw) Elem<T>::st1(d + e, acc[e]);
-                        }
+                            for (int e = 0; e < 3; ++e)
+                                if (c + e < dcw) Elem<T>::st1(d + e, acc[e]);
                     }
                 }
             }
         }
-
         oi += ostep;
 
         // ---- S = e^{g cnt} S + (w b)^T c
@@ -396,13 +378,13 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
     if (p.s_fin && seg == p.nseg - 1) each_state([&](float v, bool in, int64_t at) { if (in) p.s_fin[st_base + at] = v; return v; });
 }
 
-template <typename T, int DA, int DC, bool VEC, bool STATE> int launch(const DecayPasses &ps, hipStream_t st) {
+template <typename T, int DA, int DC, bool STATE> int launch(const DecayPasses &ps, hipStream_t st) {
     constexpr int bytes = STATE ? Lds<T, DA, DC>::STATE_BYTES : Lds<T, DA, DC>::BYTES;
     static_assert(bytes <= kMaxLds, "LDS of one CU");
     const DecayPass &p = ps.p[0];
     const int64_t blocks = (int64_t)p.n * p.H * ((p.dc + DC - 1) / DC) * (STATE ? p.nseg - 1 : p.nseg) * ps.np;
     EVFLY_REQUIRE(blocks <= INT32_MAX, "decay_attention: %lld tiles of work", (long long)blocks);
-    const auto kern = k_decay_chunk<T, DA, DC, VEC, STATE>;
+    const auto kern = k_decay_chunk<T, DA, DC, STATE>;
     static std::atomic<bool> attr_set[64];
     int dev = 0;
     EVFLY_HIP(hipGetDevice(&dev));
@@ -416,15 +398,14 @@ template <typename T, int DA, int DC, bool VEC, bool STATE> int launch(const Dec
     return 0;
 }
 
-template <typename T, int DA, int DC> int launch_v(const DecayPasses &p, bool state, bool vec, hipStream_t st) {
-    if (state) return vec ? launch<T, DA, DC, true, true>(p, st) : launch<T, DA, DC, false, true>(p, st);
-    return vec ? launch<T, DA, DC, true, false>(p, st) : launch<T, DA, DC, false, false>(p, st);
+template <typename T, int DA, int DC> int launch_s(const DecayPasses &p, bool state, hipStream_t st) {
+    return state ? launch<T, DA, DC, true>(p, st) : launch<T, DA, DC, false>(p, st);
 }
-template <typename T> int launch_all(const DecayPasses &p, bool state, bool vec, hipStream_t st) {
+template <typename T> int launch_all(const DecayPasses &p, bool state, hipStream_t st) {
     const int DA = decay_tile_a(p.p[0].da);
     if (decay_tile_c(p.p[0].dc) == 32)
-        return DA == 32 ? launch_v<T, 32, 32>(p, state, vec, st) : DA == 64 ? launch_v<T, 64, 32>(p, state, vec, st) : launch_v<T, 128, 32>(p, state, vec, st);
-    return DA == 32 ? launch_v<T, 32, 64>(p, state, vec, st) : DA == 64 ? launch_v<T, 64, 64>(p, state, vec, st) : launch_v<T, 128, 64>(p, state, vec, st);
+        return DA == 32 ? launch_s<T, 32, 32>(p, state, st) : DA == 64 ? launch_s<T, 64, 32>(p, state, st) : launch_s<T, 128, 32>(p, state, st);
+    return DA == 32 ? launch_s<T, 32, 64>(p, state, st) : DA == 64 ? launch_s<T, 64, 64>(p, state, st) : launch_s<T, 128, 64>(p, state, st);
 }
 
 }  // namespace decay
