@@ -77,13 +77,13 @@ __device__ __forceinline__ uint4 load16_any(const void *p) {
 __device__ __forceinline__ void store16_any(void *p, uint4 v) { *reinterpret_cast<u32x4_any *>(p) = u32x4_any{v.x, v.y, v.z, v.w}; }
 __device__ __forceinline__ void store8_any(void *p, uint2 v) { *reinterpret_cast<u32x2_any *>(p) = u32x2_any{v.x, v.y}; }
 
-// the 16-byte piece of a row of which `n` values are left: whole, its first n values and zeros, or nothing (n <= 0)
-template <typename T> __device__ __forceinline__ uint4 load_piece(const T *at, int n) {
+// the 16-byte piece of a row of which `n` values are left: whole, its first n values and zeros (TAIL), or nothing (n <= 0)
+template <typename T, bool TAIL> __device__ __forceinline__ uint4 load_piece(const T *at, int n) {
     constexpr int V = 16 / sizeof(T);
     if (n >= V) return load16_any(at);
     union { T v[V]; uint4 u; } r;
     r.u = make_uint4(0, 0, 0, 0);
-    if (n > 0) {
+    if (TAIL && n > 0) {
 #pragma unroll
         for (int e = 0; e < V - 1; ++e)
             if (e < n) r.v[e] = at[e];

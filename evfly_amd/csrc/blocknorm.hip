@@ -48,7 +48,7 @@ template <typename T, int G> struct Row {
 #pragma unroll
         for (int k = 0; k < E / VS<T>; ++k) {
             const int c = (k * G + gl) * VS<T>;
-            raw[k] = load_piece<T>(row + c, C - c);
+            raw[k] = load_piece<T, true>(row + c, C - c);
         }
     }
     __device__ __forceinline__ void clear() {
