@@ -9,8 +9,9 @@ namespace {
 
 // ---------------------------------------------------------------------------------------- recurrence, few tokens
 // S_t = e^g S_{t-1} + k_t v_t^T, out_t = scale q_t S_t with the state in registers from its one read to its one write: a call for one
-// window moves 8 bytes per state element and little else. One block per (stream, head); a thread holds VW neighbouring columns of the rows
-// m R + rg; the tokens' q and k wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
+// window moves 8 bytes per state element and little else. One block per (stream, head) of four waves, or of one for several tokens on a state of up to 32 x 32 (256
+// streams x 10 windows x 8 heads of 32: 11.5 us, four waves exchanging column sums 14.6; one token, 64 streams x 4 heads: 4.3 against 3.7). A thread holds VW
+// neighbouring columns of the rows m R + rg; the tokens wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
 
 struct StepArgs {
     const void *q, *k, *v;
@@ -23,16 +24,17 @@ struct StepArgs {
     float scale;
 };
 
-template <typename T, int VW, int CG> __global__ __launch_bounds__(256) void k_decay_step(StepArgs p) {
-    constexpr int R = 256 / CG, RT = EVFLY_DECAY_MAX_DIM / R;          // rows side by side; rows per thread
-    constexpr int NPART = CG <= 64 ? 4 : 2;                              // partial column sums per token
+template <typename T, int VW, int CG, int NW> __global__ __launch_bounds__(64 * NW) void k_decay_step(StepArgs p) {
+    constexpr int R = 64 * NW / CG, RT = (NW == 1 ? 32 : EVFLY_DECAY_MAX_DIM) / R;      // rows side by side; rows per thread
+    constexpr int NPART = CG <= 64 ? NW : NW / 2;                        // partial column sums per token
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG, c = cg * VW;
     const int h = blockIdx.x % p.H;
     const int64_t n = blockIdx.x / p.H;
     const int len = p.lengths ? min(max(p.lengths[n], 0), p.T) : p.T;
     const int64_t sb = (n * p.H + h) * p.dk * p.dv;
-    float *const qk = sm, *const part = sm + 2 * p.T * p.dk;
+    const int tw = 2 * p.dk + CG * VW;                                   // a token's q, k and v (v padded with zeros to the threads' columns)
+    float *const tok = sm, *const part = sm + p.T * tw;
 
     float S[RT][VW];
 #pragma unroll
@@ -49,9 +51,20 @@ template <typename T, int VW, int CG> __global__ __launch_bounds__(256) void k_d
     const T *const qp = static_cast<const T *>(p.q) + n * p.qs[0] + h * p.qs[2];
     const T *const kp = static_cast<const T *>(p.k) + n * p.ks[0] + (h / p.rep) * p.ks[2];
     const T *const vp = static_cast<const T *>(p.v) + n * p.vs[0] + (h / p.rep) * p.vs[2];
-    for (int i = tid; i < 2 * len * p.dk; i += 256) {
-        const int t = i / (2 * p.dk), r = i % (2 * p.dk);
-        qk[i] = r < p.dk ? Elem<T>::ld1(qp + t * p.qs[1] + r) : Elem<T>::ld1(kp + t * p.ks[1] + (r - p.dk));
+    // (unrolled: the loads of several tokens are in flight before the first one is needed)
+    const int sh = p.dk <= 32 ? 5 : p.dk <= 64 ? 6 : 7;
+#pragma unroll 4
+    for (int i = tid; i < len << sh; i += 64 * NW) {
+        const int t = i >> sh, r = i & ((1 << sh) - 1);
+        if (r < p.dk) {
+            tok[t * tw + r] = Elem<T>::ld1(qp + t * p.qs[1] + r);
+            tok[t * tw + p.dk + r] = Elem<T>::ld1(kp + t * p.ks[1] + r);
+        }
+    }
+#pragma unroll 4
+    for (int i = tid; i < len * (CG * VW); i += 64 * NW) {
+        const int t = i / (CG * VW), r = i % (CG * VW);
+        tok[t * tw + 2 * p.dk + r] = r < p.dv ? Elem<T>::ld1(vp + t * p.vs[1] + r) : 0.f;
     }
     const float keep = expf(p.log_decay[h]);
     __syncthreads();
@@ -59,10 +72,10 @@ template <typename T, int VW, int CG> __global__ __launch_bounds__(256) void k_d
         float v[VW], o[VW];
 #pragma unroll
         for (int e = 0; e < VW; ++e) {
-            v[e] = c < p.dv ? Elem<T>::ld1(vp + t * p.vs[1] + c + e) : 0.f;
+            v[e] = tok[t * tw + 2 * p.dk + c + e];
             o[e] = 0.f;
         }
-        const float *qt = qk + 2 * t * p.dk, *kt = qt + p.dk;
+        const float *qt = tok + t * tw, *kt = qt + p.dk;
 #pragma unroll
         for (int m = 0; m < RT; ++m) {
             const int row = m * R + rg;
@@ -94,26 +107,27 @@ template <typename T, int VW, int CG> __global__ __launch_bounds__(256) void k_d
             }
         }
     __syncthreads();
-    for (int i = tid; i < p.T * p.dv; i += 256) {
-        const int t = i / p.dv, col = i % p.dv;
-        float o = 0.f;
-        if (t < len)
+    for (int t = tid >> 6; t < p.T; t += NW)
+        for (int col = tid & 63; col < p.dv; col += 64) {
+            float o = 0.f;
+            if (t < len)
 #pragma unroll
-            for (int w = 0; w < NPART; ++w) o += part[(t * NPART + w) * (CG * VW) + col];
-        Elem<T>::st1(static_cast<T *>(p.out) + ((n * p.T + t) * p.H + h) * p.dv + col, t < len ? o * p.scale : 0.f);
-    }
+                for (int w = 0; w < NPART; ++w) o += part[(t * NPART + w) * (CG * VW) + col];
+            Elem<T>::st1(static_cast<T *>(p.out) + ((n * p.T + t) * p.H + h) * p.dv + col, t < len ? o * p.scale : 0.f);
+        }
 }
 
-template <typename T, int VW, int CG> int step_launch(const StepArgs &a, int n, hipStream_t st) {
-    const size_t lds = sizeof(float) * a.T * (2 * a.dk + (CG <= 64 ? 4 : 2) * CG * VW);
-    hipLaunchKernelGGL((k_decay_step<T, VW, CG>), dim3((unsigned)((int64_t)n * a.H)), dim3(256), lds, st, a);
+template <typename T, int VW, int CG, int NW> int step_launch(const StepArgs &a, int n, hipStream_t st) {
+    const size_t lds = sizeof(float) * a.T * (2 * a.dk + CG * VW + (CG <= 64 ? NW : NW / 2) * CG * VW);      // at most 56 KB
+    hipLaunchKernelGGL((k_decay_step<T, VW, CG, NW>), dim3((unsigned)((int64_t)n * a.H)), dim3(64 * NW), lds, st, a);
     EVFLY_LAUNCH_CHECK();
     return 0;
 }
 template <typename T> int step_all(const StepArgs &a, int n, hipStream_t st) {
     const bool v4 = a.dv % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.s_in) | reinterpret_cast<uintptr_t>(a.s_out)) & 15) == 0;
-    if (v4) return a.dv <= 32 ? step_launch<T, 4, 8>(a, n, st) : a.dv <= 64 ? step_launch<T, 4, 16>(a, n, st) : step_launch<T, 4, 32>(a, n, st);
-    return a.dv <= 32 ? step_launch<T, 1, 32>(a, n, st) : a.dv <= 64 ? step_launch<T, 1, 64>(a, n, st) : step_launch<T, 1, 128>(a, n, st);
+    if (v4 && a.T > 1 && a.dv <= 32 && a.dk <= 32) return step_launch<T, 4, 8, 1>(a, n, st);
+    if (v4) return a.dv <= 32 ? step_launch<T, 4, 8, 4>(a, n, st) : a.dv <= 64 ? step_launch<T, 4, 16, 4>(a, n, st) : step_launch<T, 4, 32, 4>(a, n, st);
+    return a.dv <= 32 ? step_launch<T, 1, 32, 4>(a, n, st) : a.dv <= 64 ? step_launch<T, 1, 64, 4>(a, n, st) : step_launch<T, 1, 128, 4>(a, n, st);
 }
 
 // ---------------------------------------------------------------------------------------- states at the segment borders

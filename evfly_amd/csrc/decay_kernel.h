@@ -150,7 +150,8 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
     constexpr int NC = DC / 16;                      // 16-column tiles of c
     constexpr int NA = DA >= 64 ? DA / 64 : 1;       // the wave's share of the state: NA a-tiles by NCW c-tiles
     constexpr int NCW = DA >= 64 ? NC : NC / 2;
-    // pairs whose weights are all zero (later tokens): fp32, bound by its products, leaves them out; in bf16 the branches around them cost more
+    // products with nothing but zeros (pairs with later tokens, tiles behind the head size): fp32, bound by its products, leaves them out; in bf16 the
+    // branches around them cost more
     constexpr bool SKIP = sizeof(T) == 4;
     constexpr int NB = C * DA / V / 256, NV = C * DC / V / 256;      // 16-byte pieces per thread of a chunk of b and c
     static_assert(NB >= 1 && NV >= 1, "a chunk is at least one piece per thread");
@@ -165,14 +166,15 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
     int id = xcd * q8 + min(xcd, r8) + blockIdx.x / kNumXCD;
     const DecayPass &p = ps.p[id % ps.np]; id /= ps.np;
     const int nseg = STATE ? p.nseg - 1 : p.nseg, ndc = (p.dc + DC - 1) / DC;
-    const int c0 = (id % ndc) * DC; id /= ndc;
+    const int wide = ((p.dc + ndc - 1) / ndc + 15) / 16 * 16;            // columns per block, evenly shared (96: 48 and 48)
+    const int c0 = (id % ndc) * wide; id /= ndc;
     const int h = id % p.H; id /= p.H;
     const int seg = id % nseg;
     const int n = id / nseg;
 
     const int len = p.lengths ? min(max(p.lengths[n], 0), p.T) : p.T;
     const int u_lo = seg * p.seg_len, u_hi = min(u_lo + p.seg_len, p.T), u_end = min(u_hi, len);
-    const int dcw = min(p.dc - c0, DC);              // columns of this tile
+    const int dcw = max(0, min(p.dc - c0, wide));    // columns of this tile
     const int o = p.rev ? 0 : 1;
     const T *const ap = static_cast<const T *>(p.a) + n * p.as[0] + (h / p.ra) * p.as[2];
     const T *const bp = static_cast<const T *>(p.b) + n * p.bs[0] + (h / p.rb) * p.bs[2];
@@ -290,7 +292,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
                     if (SKIP && st > wt) continue;
 #pragma unroll
                     for (int k = 0; k < KA; ++k)
-                        acc[x] = M::mma(M::load(lds + L::B + (16 * st + l) * L::RB + k * 64 + g * 16), fa[k], acc[x]);
+                        if (!SKIP || k * M::KB < p.da) acc[x] = M::mma(M::load(lds + L::B + (16 * st + l) * L::RB + k * 64 + g * 16), fa[k], acc[x]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[x][e] *= wp[st][e];
                 }
@@ -300,12 +302,13 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
             const bool there = u0 + ar < u_end;
 #pragma unroll
             for (int y = 0; y < NC; ++y) {
+                if (SKIP && 16 * y >= dcw) continue;
                 f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < KA; ++k)
 #pragma unroll
                     for (int x = 0; x < M::NP; ++x)
-                        acc = M::mma(M::load(lds + L::S + x * L::PLANE + (16 * y + l) * L::RS + k * 64 + g * 16), fa[k], acc);
+                        if (!SKIP || k * M::KB < p.da) acc = M::mma(M::load(lds + L::S + x * L::PLANE + (16 * y + l) * L::RS + k * 64 + g * 16), fa[k], acc);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] *= w_out;
 #pragma unroll
@@ -356,6 +359,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
             for (int x = 0; x < NA; ++x) M::weigh(M::load_col(lds + L::B, L::RB, ks, g, 16 * (a_t0 + x) + l), wu, fb[x]);
 #pragma unroll
             for (int y = 0; y < NCW; ++y) {
+                if (SKIP && 16 * (c_t0 + y) >= dcw) continue;
                 const frag fc = M::load_col(lds + L::C, L::RC, ks, g, 16 * (c_t0 + y) + l);
 #pragma unroll
                 for (int x = 0; x < NA; ++x)
