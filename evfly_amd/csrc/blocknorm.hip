@@ -8,6 +8,7 @@
 //
 // Column sums (weights, biases, residual scale, a broadcast gate) are kept per lane over the block's rows, added over the block's groups in LDS, written
 // as one partial row per block and added in block order by k_bn_columns: no atomics, the same bits on every call.
+#include <atomic>
 #include <cmath>
 
 #include "bf16.h"
@@ -283,14 +284,24 @@ template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) voi
     __shared__ float lds[NT / GW > 1 ? NT / GW * E * G : 1];
     int turn = 0;
     const int gl = threadIdx.x % G, gi = threadIdx.x / G;
+    // A block of 1024 threads has 128 registers per thread: it reads weights and rows when it needs them and keeps four of the column sums in LDS (8192
+    // channels, bf16, 4096 rows: 144 us; 466 with everything in registers, spilled, on half as many blocks)
+    constexpr bool KEEP = G < 1024;
     float w1[E], b1[E], w2[E], al[E];
-    load_vec<T, G>(p.w1, gl, p.C, 1.f, w1);
-    load_vec<T, G>(p.b1, gl, p.C, 0.f, b1);
-    load_vec<T, G>(p.w2, gl, p.C, 1.f, w2);
-    load_vec<T, G>(p.alpha, gl, p.C, 1.f, al);
-    float sa[E], sw1[E], sb1[E], sw2[E], sb2[E], sg[E];
+    if (KEEP) {
+        load_vec<T, G>(p.w1, gl, p.C, 1.f, w1);
+        load_vec<T, G>(p.b1, gl, p.C, 0.f, b1);
+        load_vec<T, G>(p.w2, gl, p.C, 1.f, w2);
+        load_vec<T, G>(p.alpha, gl, p.C, 1.f, al);
+    }
+    float sa[KEEP ? E : 1], sw1[KEEP ? E : 1], sb1[KEEP ? E : 1], sw2[KEEP ? E : 1], sb2[E], sg[E];
+    extern __shared__ float held[];                   // !KEEP: w1, b1, w2 and alpha sums, [kind][value][thread]
+    auto sum = [&](float *reg, int kind, int j) -> float & {
+        if constexpr (KEEP) return reg[j];
+        else return held[(kind * E + j) * NT + threadIdx.x];
+    };
 #pragma unroll
-    for (int j = 0; j < E; ++j) sa[j] = sw1[j] = sb1[j] = sw2[j] = sb2[j] = sg[j] = 0.f;
+    for (int j = 0; j < E; ++j) sum(sa, 3, j) = sum(sw1, 0, j) = sum(sb1, 1, j) = sum(sw2, 2, j) = sb2[j] = sg[j] = 0.f;
     const bool gate_rows = p.dgate && p.rpg > 1 && p.rpg < p.rows;        // a gate row for several rows, not for all
     for (uint32_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
         // unit = (gate row, part); its rows lie in one gate row (one gate row for everything: parts of all rows)
@@ -315,24 +326,33 @@ template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) voi
             if (p.dy) ny.fetch(static_cast<const T *>(p.dy) + r * p.C, gl, p.C);
             if (p.dh) nh.fetch(static_cast<const T *>(p.dh) + r * p.C, gl, p.C);
         };
-        fetch(lo + gi);
+        if (KEEP) fetch(lo + gi);
         for (int64_t r0 = lo; r0 < hi; r0 += GR) {
             const int64_t r = r0 + gi;
             const bool live = r < hi;
             float f[E], x[E], dy[E], dh[E];
+            if (!KEEP) {
+                nf.clear(); nx.clear(); ny.clear(); nh.clear();
+                fetch(r);
+            }
             nf.widen(f);
             nx.widen(x);
             ny.widen(dy);
             nh.widen(dh);
             if (live && p.gate && p.rpg == 1) load_act(r);
-            fetch(r + GR);
+            if (KEEP) fetch(r + GR);
             // forward again: fh = normalised f, u = its affine form
             float r1 = 1.f, u[E];
             if (p.post != EVFLY_NORM_NONE) r1 = normalise<T, G>(f, p.post, gl, p.C, p.inv_c, p.eps, red, turn);
+            if (!KEEP) {
+                load_vec<T, G>(p.w1, gl, p.C, 1.f, w1);
+                load_vec<T, G>(p.b1, gl, p.C, 0.f, b1);
+            }
 #pragma unroll
             for (int j = 0; j < E; ++j) u[j] = p.post != EVFLY_NORM_NONE ? fmaf(f[j], w1[j], b1[j]) : f[j];
             if (p.pre != EVFLY_NORM_NONE) {
                 float y[E];
+                if (!KEEP) load_vec<T, G>(p.alpha, gl, p.C, 1.f, al);
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     y[j] = a[j] * u[j];
@@ -340,11 +360,12 @@ template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) voi
                 }
                 const float r2 = normalise<T, G>(y, p.pre, gl, p.C, p.inv_c, p.eps, red, turn);
                 float s[2] = {0.f, 0.f};
+                if (!KEEP) load_vec<T, G>(p.w2, gl, p.C, 1.f, w2);
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     if (live) {                          // (a row that is not there may normalise to NaN: its zeros are not enough)
                         sb2[j] += dh[j];
-                        sw2[j] = fmaf(dh[j], y[j], sw2[j]);
+                        sum(sw2, 2, j) = fmaf(dh[j], y[j], sum(sw2, 2, j));
                     }
                     dh[j] *= w2[j];
                     s[0] += dh[j];
@@ -356,11 +377,12 @@ template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) voi
                 for (int j = 0; j < E; ++j) dy[j] = fmaf(r2, dh[j] - m0 - y[j] * m1, dy[j]);
             }
             // dy is now the gradient of y from both outputs
+            if (!KEEP) load_vec<T, G>(p.alpha, gl, p.C, 1.f, al);
             float t[E];
             if (p.x) {
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
-                    if (live) sa[j] = fmaf(dy[j], x[j], sa[j]);
+                    if (live) sum(sa, 3, j) = fmaf(dy[j], x[j], sum(sa, 3, j));
                     t[j] = al[j] * dy[j];
                 }
                 if (live && p.dx) store_row<T, G>(static_cast<T *>(p.dx) + r * p.C, gl, p.C, t);
@@ -378,12 +400,13 @@ template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) voi
                 }
             }
             if (p.post != EVFLY_NORM_NONE) {
+                if (!KEEP) load_vec<T, G>(p.w1, gl, p.C, 1.f, w1);
                 float s[2] = {0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     if (live) {
-                        sb1[j] += dy[j];
-                        sw1[j] = fmaf(dy[j], f[j], sw1[j]);
+                        sum(sb1, 1, j) += dy[j];
+                        sum(sw1, 0, j) = fmaf(dy[j], f[j], sum(sw1, 0, j));
                     }
                     dy[j] *= w1[j];
                     const float in = column<T, G>(gl, j) < p.C ? dy[j] : 0.f;
@@ -414,7 +437,14 @@ template <typename T, int G> __global__ __launch_bounds__(G > 256 ? G : 256) voi
         block_columns<G, NT>(v, lds, gl, gi);
         if (gi == 0) store_columns<T, G>(out + kind * p.C, gl, p.C, v);
     };
-    flush(K_ALPHA, sa); flush(K_W1, sw1); flush(K_B1, sb1); flush(K_W2, sw2); flush(K_B2, sb2); flush(K_GATE, sg);
+    flush(K_B2, sb2); flush(K_GATE, sg);
+    auto flush_sum = [&](int kind, float *reg, int at) {
+        float v[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = sum(reg, at, j);
+        flush(kind, v);
+    };
+    flush_sum(K_W1, sw1, 0); flush_sum(K_B1, sb1, 1); flush_sum(K_W2, sw2, 2); flush_sum(K_ALPHA, sa, 3);
 }
 
 // out_k[c] = sum over partial rows in order: 16 runs of rows per column, then the runs. blockIdx.y: the vector; in: [row][stride], column offset kind * C.
@@ -451,7 +481,20 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 template <typename T, int G> int bn_launch(const BnArgs &p, bool backward, unsigned blocks, hipStream_t st) {
     constexpr int NT = G > 256 ? G : 256;
-    if (backward) hipLaunchKernelGGL((k_bn_bwd<T, G>), dim3(blocks), dim3(NT), 0, st, p);
+    if (backward) {
+        constexpr int held = G < 1024 ? 0 : 4 * E * NT * (int)sizeof(float);
+        if (held > 0) {
+            static std::atomic<bool> attr_set[64];
+            int dev = 0;
+            EVFLY_HIP(hipGetDevice(&dev));
+            EVFLY_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
+            if (!attr_set[dev].load(std::memory_order_acquire)) {
+                EVFLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_bn_bwd<T, G>), hipFuncAttributeMaxDynamicSharedMemorySize, held));
+                attr_set[dev].store(true, std::memory_order_release);
+            }
+        }
+        hipLaunchKernelGGL((k_bn_bwd<T, G>), dim3(blocks), dim3(NT), held, st, p);
+    }
     else hipLaunchKernelGGL((k_bn_fwd<T, G>), dim3(blocks), dim3(NT), 0, st, p);
     EVFLY_LAUNCH_CHECK();
     return 0;
@@ -493,7 +536,7 @@ BnPlan bn_plan(int64_t rows, int C, int64_t rpg) {
     b.GR = (b.G > 256 ? b.G : 256) / b.G;
     const bool streams = rpg > 1 && rpg < rows;
     const int64_t span = streams ? rpg : rows, groups = streams ? rows / rpg : 1;
-    const int max_blocks = b.G > 256 ? BN_MAX_BLOCKS * 256 / b.G : BN_MAX_BLOCKS;
+    const int max_blocks = b.G > 256 ? kNumCU : BN_MAX_BLOCKS;
     int64_t parts = (max_blocks + groups - 1) / groups;
     const int64_t most = (span + 2 * b.GR - 1) / (2 * b.GR);
     if (parts > most) parts = most;
