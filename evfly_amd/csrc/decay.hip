@@ -238,7 +238,7 @@ int check_shape(const char *who, int n, int T, int H, int KV, int dk, int dv, in
     EVFLY_REQUIRE(dk > 0 && dv > 0 && dk <= EVFLY_DECAY_MAX_DIM && dv <= EVFLY_DECAY_MAX_DIM, "%s: head sizes %d, %d are not in 1 .. %d", who, dk, dv, EVFLY_DECAY_MAX_DIM);
     EVFLY_REQUIRE(dtype == EVFLY_DTYPE_F32 || dtype == EVFLY_DTYPE_BF16, "%s: dtype %d (EVFLY_DTYPE_F32 or EVFLY_DTYPE_BF16)", who, dtype);
     EVFLY_REQUIRE(std::isfinite(scale), "%s: scale is not finite", who);
-    EVFLY_REQUIRE((int64_t)n * H <= INT32_MAX, "%s: %d streams of %d heads", who, n, H);
+    EVFLY_REQUIRE((int64_t)n * H <= UINT32_MAX / 256, "%s: %d streams of %d heads", who, n, H);      // (a launch counts its threads in 32 bits)
     return 0;
 }
 

@@ -388,7 +388,7 @@ template <typename T, int DA, int DC, bool STATE, bool TAIL> int launch(const De
     static_assert(bytes <= kMaxLds, "LDS of one CU");
     const DecayPass &p = ps.p[0];
     const int64_t blocks = (int64_t)p.n * p.H * ((p.dc + DC - 1) / DC) * (STATE ? p.nseg - 1 : p.nseg) * ps.np;
-    EVFLY_REQUIRE(blocks <= INT32_MAX, "decay_attention: %lld tiles of work", (long long)blocks);
+    EVFLY_REQUIRE(blocks <= UINT32_MAX / 256, "decay_attention: %lld tiles of work", (long long)blocks);
     const auto kern = k_decay_chunk<T, DA, DC, STATE, TAIL>;
     static std::atomic<bool> attr_set[64];
     int dev = 0;

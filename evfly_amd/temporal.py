@@ -223,7 +223,8 @@ def decay_attention_step(q, k, v, log_decay, state, lengths=None, scale=None, ne
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or dst.requires_grad):
         raise ValueError(f"{who} has no gradients: call decay_attention, or wrap the call in torch.no_grad()")
     out = _decay_forward(q, k, v, log_decay, state, lengths, scale, dst)
-    torch.autograd.graph.increment_version(dst)                  # written behind autograd's back
+    if not dst.is_inference():                                   # (an inference tensor has no version)
+        torch.autograd.graph.increment_version(dst)              # written behind autograd's back
     return out
 
 

@@ -304,6 +304,80 @@ def test_decay_refusals(gpu_device):
         out.sum().backward()
 
 
+@pytest.mark.parametrize("T", [1, 5, 100])
+def test_decay_state_at_any_address(gpu_device, T):
+    """A state that starts 4 bytes behind a 16-byte boundary."""
+    from evfly_amd.temporal import decay_attention, decay_attention_step
+    d = _cuda(decay_inputs(3, T, 2, 1, 24, 32, F32, seed=19))
+    n = d["state"].numel()
+    odd = lambda: torch.zeros(n + 1, device="cuda")[1:].view(d["state"].shape)
+    S, N = odd().copy_(d["state"]), odd()
+    ref = decay_attention(d["q"], d["k"], d["v"], d["log_decay"], state=d["state"])
+    got = decay_attention(d["q"], d["k"], d["v"], d["log_decay"], state=S)
+    assert (got[0] - ref[0]).abs().max() <= 128 * EPS32 * 4 * ref[0].abs().max() and (got[1] - ref[1]).abs().max() <= 128 * EPS32 * 4 * ref[1].abs().max()
+    if T == 1:
+        out = decay_attention_step(d["q"][:, 0], d["k"][:, 0], d["v"][:, 0], d["log_decay"], S, new_state=N)
+        assert torch.equal(out, got[0][:, 0]) and torch.equal(N, got[1])
+
+
+def test_decay_in_inference_mode(gpu_device):
+    """Serving code runs under torch.inference_mode: its own tensors (which have no version) and ordinary ones."""
+    from evfly_amd.temporal import block_norm, decay_attention, decay_attention_step
+    d = _cuda(decay_inputs(2, 1, 2, 2, 16, 16, F32, seed=20))
+    q, k, v = (d[m][:, 0] for m in "qkv")
+    ref, want = decay_attention(d["q"], d["k"], d["v"], d["log_decay"], state=d["state"])
+    with torch.inference_mode():
+        for S in (d["state"].clone(), torch.empty_like(d["state"]).copy_(d["state"])):
+            out = decay_attention_step(q, k, v, d["log_decay"], S)
+            assert torch.equal(out, ref[:, 0]) and torch.equal(S, want)
+        y, h = block_norm(out, pre="rms")
+        assert torch.equal(y, out) and h.shape == out.shape
+    S = d["state"].clone()
+    with torch.inference_mode():
+        decay_attention_step(q, k, v, d["log_decay"], S)
+    assert torch.equal(S, want)
+
+
+def test_two_host_threads_on_two_streams(gpu_device):
+    """Calls from two threads at once, each on its own stream with its own tensors, give the bits of the calls made one after the other."""
+    import threading
+    from evfly_amd.temporal import block_norm, decay_attention
+    ds = [_cuda(decay_inputs(2, 700, 4, 2, 64, 64, BF16, seed=s)) for s in (21, 22)]
+
+    def work(c):
+        out, S = decay_attention(c["q"], c["k"], c["v"], c["log_decay"], state=c["state"])
+        return out, S, block_norm(out, c["q"], pre="layer")[1]
+
+    want = [work(c) for c in ds]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def run(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(10):
+                    got[i].append(work(ds[i]))
+            st.synchronize()
+        except Exception as e:                                   # (an assert in a thread would be lost)
+            errors.append(e)
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not errors
+    for i in range(2):
+        assert len(got[i]) == 10 and all(torch.equal(a, b) for r in got[i] for a, b in zip(r, want[i]))
+
+
+def test_no_second_order(gpu_device):
+    from evfly_amd.temporal import block_norm, decay_attention
+    q = torch.randn(1, 20, 1, 8, device="cuda", requires_grad=True)
+    for y in (decay_attention(q, q, q, torch.zeros(1, device="cuda"))[0], block_norm(q, pre="rms")[1]):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            torch.autograd.grad(y.sum(), q, create_graph=True)
+
+
 # ---------------------------------------------------------------------------------------- block norm
 def _norm_inputs(lead, C, dtype, gate, seed, residual=True, scale=True, offset=0.0):
     g = torch.Generator().manual_seed(seed)
