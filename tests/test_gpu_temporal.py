@@ -510,6 +510,26 @@ def test_block_norm_constant_rows(gpu_device):
     assert torch.isfinite(torch.autograd.grad(h.square().sum(), w)[0]).all()
 
 
+def test_block_norm_gate_far_out(gpu_device):
+    """Saturated gates: exact ends at +-infinity, right to some ulp of one (absolute) in between, NaN stays NaN; finite gradients wherever the value is finite."""
+    from evfly_amd.temporal import block_norm
+    z = torch.tensor([0.0, 1e-8, -1e-8, 0.5, -0.5, 10.0, -10.0, 40.0, -40.0, 79.0, -79.0, 81.0, -81.0, 88.0, -88.0, 90.0, -90.0, 104.0, -104.0, 3e38, -3e38, math.inf, -math.inf,
+                      math.nan, 20.0, -20.0, 5.0, -5.0, 1.0, -1.0, 2.0, -2.0]).view(1, 32)
+    f = torch.ones(1, 32, device="cuda", requires_grad=True)
+    for act, want in (("sigmoid", torch.sigmoid(z.double())), ("tanh", torch.tanh(z.double()))):
+        g = z.cuda().requires_grad_()
+        y, _ = block_norm(f, gate=g, gate_act=act)
+        got = y.detach().double().cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        ok = ~torch.isnan(want)
+        assert ((got - want).abs()[ok] <= 8 * EPS32).all()                     # a handful of roundings of values up to one
+        if act == "sigmoid":                                                   # and of the value itself where it is small
+            mid = ok & (z.abs() <= 79)
+            assert ((got - want).abs()[mid] <= 16 * EPS32 * want.abs()[mid]).all()
+        df, dg = torch.autograd.grad(y.sum(), [f, g])
+        assert torch.isfinite(df.cpu()[ok]).all() and torch.isfinite(dg.cpu()[ok]).all()
+
+
 def test_block_norm_no_rows_and_strides(gpu_device):
     from evfly_amd.temporal import block_norm
     w = torch.ones(16, device="cuda", requires_grad=True)
