@@ -66,6 +66,16 @@ template <> struct Elem<bf16_t> {
     __device__ static __forceinline__ void st1(bf16_t *p, float v) { *p = f2bf_dev(v); }
 };
 
+// sum over lane and lane ^ 16, lane ^ 32 (every lane gets it): the row and half swaps of gfx950 with one operand twice, no LDS cross-lane traffic
+__device__ __forceinline__ float sum_xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float sum_xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // 16 and 8 bytes at any element's address: gfx950 loads and stores them whole without alignment (a row of an odd width costs the cache lines it
 // straddles, not a load per element)
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));

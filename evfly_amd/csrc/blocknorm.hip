@@ -138,8 +138,8 @@ template <int G> __device__ __forceinline__ float lane_sum(float v) {
     if (G >= 4) v += dpp<0x4E>(v);          // quad_perm 2,3,0,1
     if (G >= 8) v += dpp<0x141>(v);         // row_half_mirror
     if (G >= 16) v += dpp<0x140>(v);        // row_mirror
-    if (G >= 32) v += __shfl_xor(v, 16);
-    if (G >= 64) v += __shfl_xor(v, 32);
+    if (G >= 32) v = sum_xor16(v);
+    if (G >= 64) v = sum_xor32(v);
     return v;
 }
 // sums of N values over the G lanes of a row. G > 64: over the group's waves through `red` (two buffers in turn: one barrier per sum; every thread of the block comes here)

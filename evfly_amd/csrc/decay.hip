@@ -11,7 +11,7 @@ namespace {
 // S_t = e^g S_{t-1} + k_t v_t^T, out_t = scale q_t S_t with the state in registers from its one read to its one write: a call for one
 // window moves 8 bytes per state element and little else. One block per (stream, head) of four waves, or of one for several tokens on a state of up to 32 x 32 (256
 // streams x 10 windows x 8 heads of 32: 11.5 us, four waves exchanging column sums 14.6; one token, 64 streams x 4 heads: 4.3 against 3.7). A thread holds VW
-// neighbouring columns of the rows m R + rg; the tokens wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
+// neighbouring columns of neighbouring rows; the tokens wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
 
 struct StepArgs {
     const void *q, *k, *v;
@@ -24,8 +24,9 @@ struct StepArgs {
     float scale;
 };
 
-template <typename T, int VW, int CG, int NW> __global__ __launch_bounds__(64 * NW) void k_decay_step(StepArgs p) {
-    constexpr int R = 64 * NW / CG, RT = (NW == 1 ? 32 : EVFLY_DECAY_MAX_DIM) / R;      // rows side by side; rows per thread
+template <typename T, int VW, int CG, int DK, int NW> __global__ __launch_bounds__(64 * NW) void k_decay_step(StepArgs p) {
+    constexpr int R = 64 * NW / CG, RT = DK / R;                             // groups of rows side by side; rows per thread
+    static_assert(RT >= 1, "every group has rows");
     constexpr int NPART = CG <= 64 ? NW : NW / 2;                        // partial column sums per token
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG, c = cg * VW;
@@ -33,13 +34,13 @@ template <typename T, int VW, int CG, int NW> __global__ __launch_bounds__(64 * 
     const int64_t n = blockIdx.x / p.H;
     const int len = p.lengths ? min(max(p.lengths[n], 0), p.T) : p.T;
     const int64_t sb = (n * p.H + h) * p.dk * p.dv;
-    const int tw = 2 * p.dk + CG * VW;                                   // a token's q, k and v (v padded with zeros to the threads' columns)
+    constexpr int tw = 2 * DK + CG * VW;                                 // a token's q, k and v, padded with zeros to the threads' rows and columns
     float *const tok = sm, *const part = sm + p.T * tw;
 
     float S[RT][VW];
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
-        const int row = m * R + rg;
+        const int row = rg * RT + m;
 #pragma unroll
         for (int e = 0; e < VW; ++e) S[m][e] = 0.f;
         if (p.s_in && row < p.dk && c < p.dv) {
@@ -52,46 +53,39 @@ template <typename T, int VW, int CG, int NW> __global__ __launch_bounds__(64 * 
     const T *const kp = static_cast<const T *>(p.k) + n * p.ks[0] + (h / p.rep) * p.ks[2];
     const T *const vp = static_cast<const T *>(p.v) + n * p.vs[0] + (h / p.rep) * p.vs[2];
     // (unrolled: the loads of several tokens are in flight before the first one is needed)
-    const int sh = p.dk <= 32 ? 5 : p.dk <= 64 ? 6 : 7;
 #pragma unroll 4
-    for (int i = tid; i < len << sh; i += 64 * NW) {
-        const int t = i >> sh, r = i & ((1 << sh) - 1);
-        if (r < p.dk) {
-            tok[t * tw + r] = Elem<T>::ld1(qp + t * p.qs[1] + r);
-            tok[t * tw + p.dk + r] = Elem<T>::ld1(kp + t * p.ks[1] + r);
-        }
+    for (int i = tid; i < len * DK; i += 64 * NW) {
+        const int t = i / DK, r = i % DK;
+        tok[t * tw + r] = r < p.dk ? Elem<T>::ld1(qp + t * p.qs[1] + r) : 0.f;
+        tok[t * tw + DK + r] = r < p.dk ? Elem<T>::ld1(kp + t * p.ks[1] + r) : 0.f;
     }
 #pragma unroll 4
     for (int i = tid; i < len * (CG * VW); i += 64 * NW) {
         const int t = i / (CG * VW), r = i % (CG * VW);
-        tok[t * tw + 2 * p.dk + r] = r < p.dv ? Elem<T>::ld1(vp + t * p.vs[1] + r) : 0.f;
+        tok[t * tw + 2 * DK + r] = r < p.dv ? Elem<T>::ld1(vp + t * p.vs[1] + r) : 0.f;
     }
     const float keep = expf(p.log_decay[h]);
     __syncthreads();
     for (int t = 0; t < len; ++t) {
-        float v[VW], o[VW];
+        float v[VW], o[VW], qq[RT], kk[RT];
+        const float *at = tok + t * tw;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) { v[e] = at[2 * DK + c + e]; o[e] = 0.f; }
+#pragma unroll
+        for (int m = 0; m < RT; ++m) { qq[m] = at[rg * RT + m]; kk[m] = at[DK + rg * RT + m]; }
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) {
+                S[m][e] = fmaf(kk[m], v[e], keep * S[m][e]);
+                o[e] = fmaf(qq[m], S[m][e], o[e]);
+            }
 #pragma unroll
         for (int e = 0; e < VW; ++e) {
-            v[e] = tok[t * tw + 2 * p.dk + c + e];
-            o[e] = 0.f;
+            if (CG <= 8) o[e] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(o[e]), 0x128, 0xf, 0xf, true));      // row_ror:8
+            if (CG <= 16) o[e] = sum_xor16(o[e]);
+            if (CG <= 32) o[e] = sum_xor32(o[e]);
         }
-        const float *qt = tok + t * tw, *kt = qt + p.dk;
-#pragma unroll
-        for (int m = 0; m < RT; ++m) {
-            const int row = m * R + rg;
-            if (row < p.dk) {
-                const float kk = kt[row], qq = qt[row];
-#pragma unroll
-                for (int e = 0; e < VW; ++e) {
-                    S[m][e] = fmaf(kk, v[e], keep * S[m][e]);
-                    o[e] = fmaf(qq, S[m][e], o[e]);
-                }
-            }
-        }
-#pragma unroll
-        for (int d = CG; d < 64; d *= 2)
-#pragma unroll
-            for (int e = 0; e < VW; ++e) o[e] += __shfl_xor(o[e], d);
         if (CG >= 64 || (tid & 63) < CG)
 #pragma unroll
             for (int e = 0; e < VW; ++e) part[(t * NPART + (CG <= 64 ? tid >> 6 : rg)) * (CG * VW) + c + e] = o[e];
@@ -99,7 +93,7 @@ template <typename T, int VW, int CG, int NW> __global__ __launch_bounds__(64 * 
     if (p.s_out)
 #pragma unroll
         for (int m = 0; m < RT; ++m) {
-            const int row = m * R + rg;
+            const int row = rg * RT + m;
             if (row < p.dk && c < p.dv) {
                 float *s = p.s_out + sb + (int64_t)row * p.dv + c;
                 if constexpr (VW == 4) Elem<float>::store(s, S[m]);
@@ -117,17 +111,20 @@ template <typename T, int VW, int CG, int NW> __global__ __launch_bounds__(64 * 
         }
 }
 
-template <typename T, int VW, int CG, int NW> int step_launch(const StepArgs &a, int n, hipStream_t st) {
-    const size_t lds = sizeof(float) * a.T * (2 * a.dk + CG * VW + (CG <= 64 ? NW : NW / 2) * CG * VW);      // at most 56 KB
-    hipLaunchKernelGGL((k_decay_step<T, VW, CG, NW>), dim3((unsigned)((int64_t)n * a.H)), dim3(64 * NW), lds, st, a);
+template <typename T, int VW, int CG, int DK, int NW> int step_launch(const StepArgs &a, int n, hipStream_t st) {
+    const size_t lds = sizeof(float) * a.T * (2 * DK + CG * VW + (CG <= 64 ? NW : NW / 2) * CG * VW);      // at most 56 KB
+    hipLaunchKernelGGL((k_decay_step<T, VW, CG, DK, NW>), dim3((unsigned)((int64_t)n * a.H)), dim3(64 * NW), lds, st, a);
     EVFLY_LAUNCH_CHECK();
     return 0;
 }
+template <typename T, int VW, int CG> int step_rows(const StepArgs &a, int n, hipStream_t st) {
+    return a.dk <= 32 ? step_launch<T, VW, CG, 32, 4>(a, n, st) : a.dk <= 64 ? step_launch<T, VW, CG, 64, 4>(a, n, st) : step_launch<T, VW, CG, 128, 4>(a, n, st);
+}
 template <typename T> int step_all(const StepArgs &a, int n, hipStream_t st) {
     const bool v4 = a.dv % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.s_in) | reinterpret_cast<uintptr_t>(a.s_out)) & 15) == 0;
-    if (v4 && a.T > 1 && a.dv <= 32 && a.dk <= 32) return step_launch<T, 4, 8, 1>(a, n, st);
-    if (v4) return a.dv <= 32 ? step_launch<T, 4, 8, 4>(a, n, st) : a.dv <= 64 ? step_launch<T, 4, 16, 4>(a, n, st) : step_launch<T, 4, 32, 4>(a, n, st);
-    return a.dv <= 32 ? step_launch<T, 1, 32, 4>(a, n, st) : a.dv <= 64 ? step_launch<T, 1, 64, 4>(a, n, st) : step_launch<T, 1, 128, 4>(a, n, st);
+    if (v4 && a.T > 1 && a.dv <= 32 && a.dk <= 32) return step_launch<T, 4, 8, 32, 1>(a, n, st);
+    if (v4) return a.dv <= 32 ? step_rows<T, 4, 8>(a, n, st) : a.dv <= 64 ? step_rows<T, 4, 16>(a, n, st) : step_rows<T, 4, 32>(a, n, st);
+    return a.dv <= 32 ? step_rows<T, 1, 32>(a, n, st) : a.dv <= 64 ? step_rows<T, 1, 64>(a, n, st) : step_rows<T, 1, 128>(a, n, st);
 }
 
 // ---------------------------------------------------------------------------------------- states at the segment borders
@@ -178,6 +175,14 @@ template <typename T> __global__ __launch_bounds__(256) void k_decay_head_sum(He
         for (int r = 0; r < p.rep; ++r) a += s[(int64_t)r * d];
         Elem<T>::st1(static_cast<T *>(p.out[y]) + i, a);
     }
+}
+
+// The recurrence costs a step per token, a chunk of 64 the same for one token as for all. Forward, us, recurrence against chunk: 256 streams x 8 heads x 64, bf16, 8
+// tokens 18 / 23, 12 tokens 25 / 23; 64 x 16 x 128, bf16, 12 tokens 39 / 43, 16 tokens 50 / 43; 256 x 8 x 32, bf16, 16 tokens 15.4 / 15.6; fp32, 256 x 8 x 64, 16 tokens
+// 31 / 39; 64 x 16 x 128, 16 tokens 51 / 113.
+bool recurrent(int tokens, int dk, int dv, int dtype) {
+    const bool quick_chunk = dtype == EVFLY_DTYPE_BF16 && (dk > 32 || dv > 32);
+    return tokens <= (quick_chunk ? 11 : EVFLY_DECAY_STEP_TOKENS);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -315,7 +320,7 @@ extern "C" int evfly_decay_attention_forward(const void *q, const void *k, const
     token_strides(strides_host, tokens, heads, dk, tq.s);
     token_strides(strides_host ? strides_host + 3 : nullptr, tokens, kv_heads, dk, tk.s);
     token_strides(strides_host ? strides_host + 6 : nullptr, tokens, kv_heads, dv, tv.s);
-    if (tokens <= EVFLY_DECAY_STEP_TOKENS) {
+    if (recurrent(tokens, dk, dv, dtype)) {
         StepArgs a;
         a.q = q; a.k = k; a.v = v;
         for (int i = 0; i < 3; ++i) { a.qs[i] = tq.s[i]; a.ks[i] = tk.s[i]; a.vs[i] = tv.s[i]; }

@@ -158,9 +158,9 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
     extern __shared__ __align__(16) char lds[];
     float *const pw = reinterpret_cast<float *>(lds + L::PW), *const uw = reinterpret_cast<float *>(lds + L::UW);
 
-    // (every other block hands its tokens to the waves in the opposite order: later tokens have more pairs)
+    // (the waves' shares of the tokens turn with the block: later tokens have more pairs, and a last chunk may have only early ones)
     const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, g = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wt = SKIP && (blockIdx.x / kNumXCD & 1) ? 3 - w : w;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wt = (w + blockIdx.x / kNumXCD) & 3;
     // blocks of one XCD (block index mod 8) take neighbouring work: the heads of a token share cache lines, shared heads and column tiles share rows
     const int total = gridDim.x, q8 = total / kNumXCD, r8 = total % kNumXCD, xcd = blockIdx.x % kNumXCD;
     int id = xcd * q8 + min(xcd, r8) + blockIdx.x / kNumXCD;
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
         __syncthreads();
         if (u0 + C < u_end) fetch(u0 + C);
 
-        if (!STATE) {
+        if (!STATE && 16 * wt < cnt) {
             // ---- P^T tiles of this wave's tokens (j-tiles up to its own), weighted, as operand parts
             frag P[KS][M::NP];
 #pragma unroll
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
                 }
             }
         }
-        oi += ostep;
+        if (!STATE) oi += ostep;
 
         // ---- S = e^{g cnt} S + (w b)^T c
         const float keep = pw[cnt];
@@ -351,6 +351,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
                 for (int e = 0; e < 4; ++e) S[x][y][e] *= keep;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
+            if (SKIP && ks * M::KB >= cnt) continue;
             float wu[M::TILES * 4];
 #pragma unroll
             for (int e = 0; e < M::TILES * 4; ++e) wu[e] = uw[C - cnt + 16 * (ks * M::TILES + e / 4) + 4 * g + e % 4];

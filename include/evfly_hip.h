@@ -357,8 +357,8 @@ int evfly_model_profile_reset(evfly_model *m);
  * lengths (n_streams) int32 or NULL: stream i has lengths[i] tokens (taken into [0, tokens]); what q, k, v hold behind them is
  * not read, out is zero there, and state_out is the state after the stream's last token (a stream of no tokens keeps its state).
  * Inside a sequence a non-finite k or v reaches every later token, and may reach the earlier tokens of its own group of 64.
- * Up to EVFLY_DECAY_STEP_TOKENS tokens (one window per stream is the serving form) run as the recurrence with the state in registers and need
- * no workspace, longer ones in chunks of 64 on the matrix cores. workspace: at least
+ * A few tokens (one window per stream is the serving form) run as the recurrence with the state in registers, more of them in
+ * chunks of 64 on the matrix cores; up to EVFLY_DECAY_STEP_TOKENS need no workspace. workspace: at least
  * evfly_decay_attention_workspace_bytes(..., backward = 0) bytes (may be 0: workspace NULL), 16-byte aligned; one per call in
  * flight. What it holds before the call does not matter. */
 #define EVFLY_DECAY_MAX_DIM 128
