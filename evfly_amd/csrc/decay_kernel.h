@@ -7,10 +7,13 @@
 // others. All four products run on 16x16 MFMAs with token columns: P^T = b a^T leaves, in a lane, pair weights of one token i against
 // four neighbouring j, which is the operand layout of out^T = c^T P^T -- the pair products never leave registers.
 //
-// Work: one block of four waves per (stream, head, tile of DC columns of c, segment); wave w owns the chunk's tokens 16 w .. 16 w + 15
-// of the output and a share of the state's a-rows. The a rows go from memory to the wave's registers, b and c through LDS (read as rows for P, as
-// columns for the other two products), S lives in the accumulators and is copied to LDS once per chunk as an operand of a_i S. The next chunk's rows
-// are in flight during the products.
+// Work: one block of four waves per (stream, head, tile of DC columns of c, segment); wave w owns 16 of the chunk's tokens of the output and a share of
+// the state's a-rows. The a rows go from memory to the wave's registers, b and c through LDS (read as rows for P, as columns for the other two
+// products), S lives in the accumulators and is copied to LDS once per chunk as an operand of a_i S. The next chunk's rows are in flight during the products.
+//
+// Bounds. bf16, 64 wide (8 x 4096 tokens x 16 heads): a pass moves 268 MB in 70 us, 3.8 TB/s of the 4.9 that a copy reaches here. bf16, 128 wide
+// (1 x 32768 x 16): 178 us; counted busy are the matrix pipes 31 %, vector issue 52 %, LDS 53 % of the time: two waves per SIMD (61 KB of LDS a block)
+// overlap them only in part. fp32: the 16x16x4 products, 43 % of their pipe's time at 48 / 96 wide with two blocks a CU.
 #pragma once
 #include "bf16.h"
 #include "decay.h"
@@ -278,6 +281,9 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
         __syncthreads();
         if (u0 + C < u_end) fetch(u0 + C);
 
+        // (a wave that forms its output goes ahead of one that updates its state: of two waves on a SIMD one then feeds the matrix pipe while the other does
+        // its vector work; 32768 x 16 heads x 128, bf16, 282 -> 273 us, 8 x 4096 x 16 x 64 with gradients 311 -> 304)
+        __builtin_amdgcn_s_setprio(1);
         if (!STATE && 16 * wt < cnt) {
             // ---- P^T tiles of this wave's tokens (j-tiles up to its own), weighted, as operand parts
             frag P[KS][M::NP];
@@ -339,6 +345,7 @@ __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_de
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (!STATE) oi += ostep;
 
         // ---- S = e^{g cnt} S + (w b)^T c
