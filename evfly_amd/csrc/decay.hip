@@ -1,5 +1,6 @@
 // Decay attention: entry points, the plan of the chunked passes, the recurrent kernel for few tokens and the sum over shared heads.
 #include <cmath>
+#include <type_traits>
 
 #include "bf16.h"
 #include "decay.h"
@@ -10,8 +11,8 @@ namespace {
 // ---------------------------------------------------------------------------------------- recurrence, few tokens
 // S_t = e^g S_{t-1} + k_t v_t^T, out_t = scale q_t S_t with the state in registers from its one read to its one write: a call for one
 // window moves 8 bytes per state element and little else. One block per (stream, head) of four waves, or of one for several tokens on a state of up to 32 x 32 (256
-// streams x 10 windows x 8 heads of 32: 11.5 us, four waves exchanging column sums 14.6; one token, 64 streams x 4 heads: 4.3 against 3.7). A thread holds VW
-// neighbouring columns of neighbouring rows; the tokens wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
+// streams x 10 windows x 8 heads of 32: 11.5 us, four waves exchanging column sums 14.6; one token, 64 streams x 4 heads: 4.3 against 3.7). A thread holds four
+// neighbouring columns (16 bytes at any address) of neighbouring rows; the tokens wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
 
 struct StepArgs {
     const void *q, *k, *v;
@@ -24,10 +25,9 @@ struct StepArgs {
     float scale;
 };
 
-template <typename T, int VW, int CG, int DK, int NW> __global__ __launch_bounds__(64 * NW) void k_decay_step(StepArgs p) {
-    constexpr int R = 64 * NW / CG, RT = DK / R;                             // groups of rows side by side; rows per thread
+template <typename T, int CG, int DK, int NW> __global__ __launch_bounds__(64 * NW) void k_decay_step(StepArgs p) {
+    constexpr int VW = 4, R = 64 * NW / CG, RT = DK / R;                             // groups of rows side by side; rows per thread
     static_assert(RT >= 1, "every group has rows");
-    constexpr int NPART = CG <= 64 ? NW : NW / 2;                        // partial column sums per token
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG, c = cg * VW;
     const int h = blockIdx.x % p.H;
@@ -38,17 +38,22 @@ template <typename T, int VW, int CG, int DK, int NW> __global__ __launch_bounds
     float *const tok = sm, *const part = sm + p.T * tw;
 
     float S[RT][VW];
+    auto read_state = [&](auto tail) {                                   // (a width of whole pieces: every load free of the others' branches)
 #pragma unroll
-    for (int m = 0; m < RT; ++m) {
-        const int row = rg * RT + m;
-#pragma unroll
-        for (int e = 0; e < VW; ++e) S[m][e] = 0.f;
-        if (p.s_in && row < p.dk && c < p.dv) {
-            const float *s = p.s_in + sb + (int64_t)row * p.dv + c;
-            if constexpr (VW == 4) Elem<float>::load(s, S[m]);
-            else S[m][0] = *s;
+        for (int m = 0; m < RT; ++m) {
+            const int row = rg * RT + m;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (row < p.dk) u = load_piece<float, decltype(tail)::value>(p.s_in + sb + (int64_t)row * p.dv + c, p.dv - c);
+            S[m][0] = __uint_as_float(u.x); S[m][1] = __uint_as_float(u.y); S[m][2] = __uint_as_float(u.z); S[m][3] = __uint_as_float(u.w);
         }
-    }
+    };
+    if (!p.s_in)
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) S[m][e] = 0.f;
+    else if (p.dv % VW == 0) read_state(std::false_type{});
+    else read_state(std::true_type{});
     const T *const qp = static_cast<const T *>(p.q) + n * p.qs[0] + h * p.qs[2];
     const T *const kp = static_cast<const T *>(p.k) + n * p.ks[0] + (h / p.rep) * p.ks[2];
     const T *const vp = static_cast<const T *>(p.v) + n * p.vs[0] + (h / p.rep) * p.vs[2];
@@ -84,21 +89,23 @@ template <typename T, int VW, int CG, int DK, int NW> __global__ __launch_bounds
         for (int e = 0; e < VW; ++e) {
             if (CG <= 8) o[e] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(o[e]), 0x128, 0xf, 0xf, true));      // row_ror:8
             if (CG <= 16) o[e] = sum_xor16(o[e]);
-            if (CG <= 32) o[e] = sum_xor32(o[e]);
+            o[e] = sum_xor32(o[e]);
         }
-        if (CG >= 64 || (tid & 63) < CG)
+        if ((tid & 63) < CG)
 #pragma unroll
-            for (int e = 0; e < VW; ++e) part[(t * NPART + (CG <= 64 ? tid >> 6 : rg)) * (CG * VW) + c + e] = o[e];
+            for (int e = 0; e < VW; ++e) part[(t * NW + (tid >> 6)) * (CG * VW) + c + e] = o[e];
     }
     if (p.s_out)
 #pragma unroll
         for (int m = 0; m < RT; ++m) {
             const int row = rg * RT + m;
-            if (row < p.dk && c < p.dv) {
-                float *s = p.s_out + sb + (int64_t)row * p.dv + c;
-                if constexpr (VW == 4) Elem<float>::store(s, S[m]);
-                else *s = S[m][0];
-            }
+            if (row >= p.dk) continue;
+            float *s = p.s_out + sb + (int64_t)row * p.dv + c;
+            if (c + 4 <= p.dv) store16_any(s, make_uint4(__float_as_uint(S[m][0]), __float_as_uint(S[m][1]), __float_as_uint(S[m][2]), __float_as_uint(S[m][3])));
+            else
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (c + e < p.dv) s[e] = S[m][e];
         }
     __syncthreads();
     for (int t = tid >> 6; t < p.T; t += NW)
@@ -106,25 +113,23 @@ template <typename T, int VW, int CG, int DK, int NW> __global__ __launch_bounds
             float o = 0.f;
             if (t < len)
 #pragma unroll
-                for (int w = 0; w < NPART; ++w) o += part[(t * NPART + w) * (CG * VW) + col];
+                for (int w = 0; w < NW; ++w) o += part[(t * NW + w) * (CG * VW) + col];
             Elem<T>::st1(static_cast<T *>(p.out) + ((n * p.T + t) * p.H + h) * p.dv + col, t < len ? o * p.scale : 0.f);
         }
 }
 
-template <typename T, int VW, int CG, int DK, int NW> int step_launch(const StepArgs &a, int n, hipStream_t st) {
-    const size_t lds = sizeof(float) * a.T * (2 * DK + CG * VW + (CG <= 64 ? NW : NW / 2) * CG * VW);      // at most 56 KB
-    hipLaunchKernelGGL((k_decay_step<T, VW, CG, DK, NW>), dim3((unsigned)((int64_t)n * a.H)), dim3(64 * NW), lds, st, a);
+template <typename T, int CG, int DK, int NW> int step_launch(const StepArgs &a, int n, hipStream_t st) {
+    const size_t lds = sizeof(float) * a.T * (2 * DK + CG * 4 + NW * CG * 4);      // at most 56 KB
+    hipLaunchKernelGGL((k_decay_step<T, CG, DK, NW>), dim3((unsigned)((int64_t)n * a.H)), dim3(64 * NW), lds, st, a);
     EVFLY_LAUNCH_CHECK();
     return 0;
 }
-template <typename T, int VW, int CG> int step_rows(const StepArgs &a, int n, hipStream_t st) {
-    return a.dk <= 32 ? step_launch<T, VW, CG, 32, 4>(a, n, st) : a.dk <= 64 ? step_launch<T, VW, CG, 64, 4>(a, n, st) : step_launch<T, VW, CG, 128, 4>(a, n, st);
+template <typename T, int CG> int step_rows(const StepArgs &a, int n, hipStream_t st) {
+    return a.dk <= 32 ? step_launch<T, CG, 32, 4>(a, n, st) : a.dk <= 64 ? step_launch<T, CG, 64, 4>(a, n, st) : step_launch<T, CG, 128, 4>(a, n, st);
 }
 template <typename T> int step_all(const StepArgs &a, int n, hipStream_t st) {
-    const bool v4 = a.dv % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.s_in) | reinterpret_cast<uintptr_t>(a.s_out)) & 15) == 0;
-    if (v4 && a.T > 1 && a.dv <= 32 && a.dk <= 32) return step_launch<T, 4, 8, 32, 1>(a, n, st);
-    if (v4) return a.dv <= 32 ? step_rows<T, 4, 8>(a, n, st) : a.dv <= 64 ? step_rows<T, 4, 16>(a, n, st) : step_rows<T, 4, 32>(a, n, st);
-    return a.dv <= 32 ? step_rows<T, 1, 32>(a, n, st) : a.dv <= 64 ? step_rows<T, 1, 64>(a, n, st) : step_rows<T, 1, 128>(a, n, st);
+    if (a.T > 1 && a.dv <= 32 && a.dk <= 32) return step_launch<T, 8, 32, 1>(a, n, st);
+    return a.dv <= 32 ? step_rows<T, 8>(a, n, st) : a.dv <= 64 ? step_rows<T, 16>(a, n, st) : step_rows<T, 32>(a, n, st);
 }
 
 // ---------------------------------------------------------------------------------------- states at the segment borders
