@@ -10,10 +10,10 @@ namespace {
 
 // ---------------------------------------------------------------------------------------- recurrence, few tokens
 // S_t = e^g S_{t-1} + k_t v_t^T, out_t = scale q_t S_t with the state in registers from its one read to its one write: a call for one
-// window moves 8 bytes per state element and little else. One block per (stream, head) of four waves, or of one for several tokens on a state of up to 32 x 32 (256
-// streams x 10 windows x 8 heads of 32: 11.5 us, four waves exchanging column sums 14.6; one token, 64 streams x 4 heads: 4.3 against 3.7). A thread holds four
-// neighbouring columns (16 bytes at any address) of neighbouring rows; the tokens wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
-
+// window moves 8 bytes per state element and little else (256 streams x 16 heads x 64 x 64: 134 MB in 23 us). One block per (stream, head) of four waves, or of
+// one for several tokens on a state of up to 32 x 32 (256 streams x 10 windows x 8 heads of 32: 12.4 us against 14.6 for four waves that exchange column sums, 10.4
+// since the tokens' loads overlap; one token, 64 streams x 4 heads: 4.3 against 3.7). A thread holds four neighbouring columns (16 bytes at any address) of
+// neighbouring rows; the tokens wait in LDS as fp32; column sums meet by lane exchange, then over the waves in LDS, once per call.
 struct StepArgs {
     const void *q, *k, *v;
     int64_t qs[3], ks[3], vs[3];
@@ -197,6 +197,7 @@ struct Tokens {              // one token tensor: pointer, element strides, head
     int64_t s[3];
     int r, d;
 };
+
 // One call's passes: roles filled in, tiles chosen, launched together where the tiles agree.
 struct Run {
     int dtype;
