@@ -21,6 +21,7 @@ MAX_HEAD_DIM = 128
 MAX_CHANNELS = 8192
 STEP_TOKENS = 16                    # up to here a forward needs no workspace (EVFLY_DECAY_STEP_TOKENS)
 _NORM = {None: 0, "layer": 1, "rms": 2}
+_GATE_ACT = {a: _lib.ACT_CODES[a] for a in ("none", "sigmoid", "tanh")}
 
 
 _getDevice, _rawStream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream      # (a tick's call is a few microseconds: no Stream object for it)
@@ -32,16 +33,6 @@ def _ptr(t):
 
 def _dense(t):
     return None if t is None else t.contiguous()
-
-
-def _on_its_device(fn):
-    """`fn(t, ...)` with t's device as the current one (it usually is)."""
-    def call(t, *args):
-        if t.get_device() == _getDevice():
-            return fn(t, *args)
-        with torch.cuda.device(t.device):
-            return fn(t, *args)
-    return call
 
 
 def _workspace(nbytes, like):
@@ -119,45 +110,62 @@ def _rows(t):
 
 
 def _strides(q, k, v):
-    if q.is_contiguous() and k.is_contiguous() and v.is_contiguous():
-        return None
     if q.dim() == 3:                                             # one token: its stride is never taken
         return (C.c_int64 * 9)(*(s for t in (q, k, v) for s in (t.stride(0), 0, t.stride(1))))
     return (C.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
 
 
-@_on_its_device
 def _decay_forward(q, k, v, log_decay, state, lengths, scale, new_state):
-    n, H, dk, KV, dv = q.shape[0], q.shape[-2], q.shape[-1], k.shape[-2], v.shape[-1]
-    T = q.shape[1] if q.dim() == 4 else 1
-    q, k, v, log_decay, state, lengths = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), _dense(state), _dense(lengths)
-    dt = _DTYPE[q.dtype]
+    idx = q.get_device()
+    if idx != _getDevice():
+        with torch.cuda.device(idx):
+            return _decay_forward(q, k, v, log_decay, state, lengths, scale, new_state)
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    n, H, dk, KV, dv = qs[0], qs[-2], qs[-1], ks[-2], v.shape[-1]
+    T = qs[1] if len(qs) == 4 else 1
+    strides = None
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        strides = _strides(q, k, v)
+    log_decay = log_decay.contiguous()
+    if state is not None:
+        state = state.contiguous()
+    if lengths is not None:
+        lengths = lengths.contiguous()
+    dt = _DTYPE[dtype]
     L = _lib.load_library()
-    out = torch.empty((*q.shape[:-1], dv), dtype=q.dtype, device=q.device)
+    out = torch.empty(qs[:-1] + (dv,), dtype=dtype, device=q.device)
     nb, ws = 0, None
     if T > STEP_TOKENS:
         nb = _lib.check(L.evfly_decay_attention_workspace_bytes(n, T, H, KV, dk, dv, dt, 0))
         ws = _workspace(nb, q)
     _lib.check(L.evfly_decay_attention_forward(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), log_decay.data_ptr(), _ptr(state), _ptr(lengths), n, T, H, KV, dk, dv, scale, dt,
-        out.data_ptr(), new_state.data_ptr(), _ptr(ws), nb, _rawStream(q.get_device())))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, log_decay.data_ptr(), state.data_ptr() if state is not None else None,
+        lengths.data_ptr() if lengths is not None else None, n, T, H, KV, dk, dv, scale, dt, out.data_ptr(), new_state.data_ptr(),
+        ws.data_ptr() if ws is not None else None, nb, _rawStream(idx)))
     return out
 
 
-@_on_its_device
 def _decay_backward(q, k, v, log_decay, state, lengths, scale, d_out, d_state, want_state):
+    if q.get_device() != _getDevice():
+        with torch.cuda.device(q.device):
+            return _decay_backward(q, k, v, log_decay, state, lengths, scale, d_out, d_state, want_state)
     n, T, H, dk = q.shape
     KV, dv = v.shape[2], v.shape[3]
     dt = _DTYPE[q.dtype]
     L = _lib.load_library()
     d_out = torch.zeros((n, T, H, dv), dtype=q.dtype, device=q.device) if d_out is None else d_out.contiguous()
     dq, dk_, dv_ = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    q, k, v, log_decay, state, lengths, d_state = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), _dense(state), _dense(lengths), _dense(d_state)
+    strides = None
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        strides = _strides(q, k, v)
+    log_decay, state, lengths, d_state = log_decay.contiguous(), _dense(state), _dense(lengths), _dense(d_state)
     ds = torch.empty_like(state) if want_state else None
     nb = _lib.check(L.evfly_decay_attention_workspace_bytes(n, T, H, KV, dk, dv, dt, 1))
     ws = _workspace(nb, q)
     _lib.check(L.evfly_decay_attention_backward(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), log_decay.data_ptr(), _ptr(state), _ptr(lengths), d_out.data_ptr(), _ptr(d_state),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, log_decay.data_ptr(), _ptr(state), _ptr(lengths), d_out.data_ptr(), _ptr(d_state),
         n, T, H, KV, dk, dv, scale, dt, dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(), _ptr(ds), _ptr(ws), nb, _rawStream(q.get_device())))
     return dq, dk_, dv_, ds
 
@@ -243,21 +251,28 @@ def _gate_rows(f, gate):
                      f"dimension and 1 from there on)")
 
 
-@_on_its_device
 def _block_forward(f, x, gate, res_scale, w1, b1, w2, b2, opt):
+    idx = f.get_device()
+    if idx != _getDevice():
+        with torch.cuda.device(idx):
+            return _block_forward(f, x, gate, res_scale, w1, b1, w2, b2, opt)
     rows_per_gate, gate_f32, act, post, pre, eps = opt
-    f, x, gate, res_scale, w1, b1, w2, b2 = f.contiguous(), _dense(x), _dense(gate), _dense(res_scale), _dense(w1), _dense(b1), _dense(w2), _dense(b2)
+    f = f.contiguous()
+    ins = [t if t is None or t.is_contiguous() else t.contiguous() for t in (x, gate, res_scale, w1, b1, w2, b2)]
+    px, pg, pa, p1, q1, p2, q2 = [None if t is None else t.data_ptr() for t in ins]
     Cn = f.shape[-1]
     y = torch.empty_like(f)
     h = torch.empty_like(f) if pre else None
     _lib.check(_lib.load_library().evfly_block_norm_forward(
-        f.data_ptr(), _ptr(x), _ptr(gate), rows_per_gate, gate_f32, act, _ptr(res_scale), post, _ptr(w1), _ptr(b1), pre, _ptr(w2), _ptr(b2), eps,
-        f.numel() // Cn, Cn, _DTYPE[f.dtype], y.data_ptr(), _ptr(h), _rawStream(f.get_device())))
+        f.data_ptr(), px, pg, rows_per_gate, gate_f32, act, pa, post, p1, q1, pre, p2, q2, eps, f.numel() // Cn, Cn, _DTYPE[f.dtype], y.data_ptr(),
+        h.data_ptr() if pre else None, _rawStream(idx)))
     return y, h
 
 
-@_on_its_device
 def _block_backward(f, x, gate, res_scale, w1, b1, w2, b2, opt, dy, dh, need):
+    if f.get_device() != _getDevice():
+        with torch.cuda.device(f.device):
+            return _block_backward(f, x, gate, res_scale, w1, b1, w2, b2, opt, dy, dh, need)
     rows_per_gate, gate_f32, act, post, pre, eps = opt
     f, x, gate, res_scale, w1, b1, w2, b2, dy, dh = (f.contiguous(), _dense(x), _dense(gate), _dense(res_scale), _dense(w1), _dense(b1), _dense(w2), _dense(b2),
                                                      _dense(dy), _dense(dh))
@@ -298,6 +313,46 @@ class _BlockNorm(torch.autograd.Function):
         return _block_backward(*ctx.saved_tensors, ctx.opt, dy, dh, ctx.needs_input_grad)
 
 
+def _block_fits(f, x, gate, gate_act, res_scale, post, w1, b1, pre, w2, b2):
+    """Everything `_refuse_block` asks for, in one look."""
+    try:
+        dt, dev, shape = f.dtype, f.device, f.shape
+        vec = shape[-1:]
+        if not (0 < vec[0] <= MAX_CHANNELS and dt in _DTYPE and dev.type == "cuda" and post in _NORM and pre in _NORM and gate_act in _GATE_ACT and
+                (x is None or (x.dtype is dt and x.device == dev and x.shape == shape)) and (x is not None or res_scale is None) and
+                (post is not None or (w1 is None and b1 is None)) and (pre is not None or (w2 is None and b2 is None)) and
+                (gate is None or ((gate.dtype is dt or gate.dtype is torch.float32) and gate.device == dev))):
+            return False
+        for t in (res_scale, w1, b1, w2, b2):
+            if t is not None and (t.dtype is not torch.float32 or t.shape != vec or t.device != dev):
+                return False
+        return True
+    except (AttributeError, IndexError, TypeError):
+        return False
+
+
+def _refuse_block(f, x, gate, gate_act, res_scale, post, w1, b1, pre, w2, b2):
+    who = "block_norm"
+    if not isinstance(f, torch.Tensor) or f.dim() < 1 or not 1 <= f.shape[-1] <= MAX_CHANNELS:
+        raise ValueError(f"{who}: f must be a tensor (..., channels) of 1 .. {MAX_CHANNELS} channels")
+    _check_tokens(who, (("f", f),) if x is None else (("f", f), ("x", x)), f)
+    if x is not None and x.shape != f.shape:
+        raise ValueError(f"{who}: x {tuple(x.shape)} is not shaped like f {tuple(f.shape)}")
+    if not all(n is None or isinstance(n, str) for n in (post, pre)) or post not in _NORM or pre not in _NORM:
+        raise ValueError(f"{who}: norms {post!r}, {pre!r} (\"layer\", \"rms\" or None)")
+    if res_scale is not None and x is None:
+        raise ValueError(f"{who}: res_scale without a residual x")
+    for kind, name, t in ((True, "res_scale", res_scale), (post, "post_weight", w1), (post, "post_bias", b1), (pre, "pre_weight", w2), (pre, "pre_bias", b2)):
+        if t is not None:
+            if not kind:
+                raise ValueError(f"{who}: {name} without a norm")
+            _check_f32(who, name, t, f.shape[-1:], f.device)
+    if not isinstance(gate_act, str) or gate_act not in _GATE_ACT:
+        raise ValueError(f"{who}: gate_act {gate_act!r} (\"none\", \"sigmoid\" or \"tanh\")")
+    if gate is not None and (not isinstance(gate, torch.Tensor) or gate.dtype not in (f.dtype, torch.float32) or gate.device != f.device):
+        raise ValueError(f"{who}: gate must be a {f.dtype} or float32 tensor on {f.device}")
+
+
 def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None, post_weight=None, post_bias=None,
                pre=None, pre_weight=None, pre_bias=None, eps=1e-5):
     """y = res_scale * x + act(gate) * norm_post(f) and h = norm_pre(y) in one pass per token; returns (y, h), h None without `pre`.
@@ -308,35 +363,15 @@ def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None,
     weight and bias (channels,) float32 or None. h is formed from y before y is rounded to the tokens' type. Gradients to every tensor.
     post=None, pre="layer" without a gate is evfly's LayerNorm(x + f)."""
     _lib.lib()
-    if not isinstance(f, torch.Tensor) or f.dim() < 1 or not 1 <= f.shape[-1] <= MAX_CHANNELS:
-        raise ValueError(f"block_norm: f must be a tensor (..., channels) of 1 .. {MAX_CHANNELS} channels")
-    dt, dev, vec = f.dtype, f.device, f.shape[-1:]
-    if dt not in _DTYPE or dev.type != "cuda" or (x is not None and not (isinstance(x, torch.Tensor) and x.dtype is dt and x.device == dev)):
-        _check_tokens("block_norm", (("f", f),) if x is None else (("f", f), ("x", x)), f)
-    if x is not None and x.shape != f.shape:
-        raise ValueError(f"block_norm: x {tuple(x.shape)} is not shaped like f {tuple(f.shape)}")
-    if post not in _NORM or pre not in _NORM:
-        raise ValueError(f"block_norm: norms {post!r}, {pre!r} (\"layer\", \"rms\" or None)")
-    if res_scale is not None and x is None:
-        raise ValueError("block_norm: res_scale without a residual x")
-    for kind, name, t in ((True, "res_scale", res_scale), (post, "post_weight", post_weight), (post, "post_bias", post_bias),
-                          (pre, "pre_weight", pre_weight), (pre, "pre_bias", pre_bias)):
-        if t is not None:
-            if not kind:
-                raise ValueError(f"block_norm: {name} without a norm")
-            if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == vec and t.device == dev):
-                _check_f32("block_norm", name, t, vec, dev)
-    if gate_act not in ("none", "sigmoid", "tanh"):
-        raise ValueError(f"block_norm: gate_act {gate_act!r} (\"none\", \"sigmoid\" or \"tanh\")")
+    if not _block_fits(f, x, gate, gate_act, res_scale, post, post_weight, post_bias, pre, pre_weight, pre_bias):
+        _refuse_block(f, x, gate, gate_act, res_scale, post, post_weight, post_bias, pre, pre_weight, pre_bias)
     eps = float(eps)
     if not (math.isfinite(eps) and eps >= 0.0):
         raise ValueError("block_norm: eps is negative or not finite")
-    rows_per_gate = 1
+    rows_per_gate, gate_f32 = 1, 0
     if gate is not None:
-        if not isinstance(gate, torch.Tensor) or gate.dtype not in (f.dtype, torch.float32) or gate.device != f.device:
-            raise ValueError(f"block_norm: gate must be a {f.dtype} or float32 tensor on {f.device}")
-        rows_per_gate = max(1, _gate_rows(f, gate))
-    opt = (rows_per_gate, int(gate is not None and gate.dtype is torch.float32), _lib.ACT_CODES[gate_act], _NORM[post], _NORM[pre], eps)
+        rows_per_gate, gate_f32 = max(1, _gate_rows(f, gate)), int(gate.dtype is torch.float32)
+    opt = (rows_per_gate, gate_f32, _GATE_ACT[gate_act], _NORM[post], _NORM[pre], eps)
     if torch.is_grad_enabled():
         for t in (f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias):
             if t is not None and t.requires_grad:
