@@ -261,12 +261,13 @@ void token_strides(const int64_t *s, int T, int heads, int d, int64_t (&out)[3])
 }  // namespace
 
 // Segments of a sequence. More of them fill the CUs and shorten the longest chain of chunks, but each cut makes two of the token tensors read twice (the state
-// pass, 0.4 of a chunk's work) and adds two launches. The split with the smallest estimate is taken:
-//     chunks per segment * t * max(1, share * blocks per CU), for each launch of the pass and, at 0.4 t, for the state pass, plus 10 us if it is cut at all
-// with t the time of a lone block's chunk (by type and a dimension) and `share` what a block uses of its CU. Measured against sweeps of 1 .. 16 blocks per CU on
-// eleven shapes; us forward / backward, chosen and the neighbours: 8 x 4096 x 16 heads x 64 bf16, four segments 96 forward (two 132, eight 105), two
-// 203 backward (four 213, eight 226); 16 x 2048 x 16 x 64 bf16, one 91 / 156 (two 97 / 198); 6 x 500 x 8 x 40 / 72 fp32, eight 35 / 89 (four 40 / 97, two 46 / 98);
-// 64 x 300 x 8 x 64 bf16, one 25 / 47 (two 45 / 86).
+// pass, 0.4 of a chunk's work) and adds two launches. The split with the smallest estimate, in us, is taken:
+//     (chunks per segment + 1/2) * t * max(1, share * blocks per CU)      for each launch of the pass and, at 0.4 t, for the state pass
+//     + 5 + 0.15 * segments                                               if it is cut at all (the scan over the borders)
+// with t the time of a lone block's chunk (by type and a dimension) and `share` what a block uses of its CU. Against sweeps of 1 .. 64 segments on thirteen shapes, forward and
+// backward, the choice is within 10 % of the best; us forward / backward, chosen and neighbours: 8 x 4096 tokens x 16 heads x 64 bf16, four 99 forward (two 133,
+// eight 104), two 198 backward (one 219, four 218); 1 x 16384 x 4 x 64 bf16, 64 segments 49 forward (16: 75); 1 x 32768 x 16 x 128 bf16, 16 segments 258 (8: 330, 32: 270); 6 x
+// 500 x 8 x 40 / 72 fp32, eight 33 / 82 (four 37 / 89, one 52 / 129); 16 x 1000 x 8 x 32 bf16, four 25 forward (one 27), one 33 backward (two 37).
 namespace {
 int col_tiles(int c) { return (c + decay_tile_c(c) - 1) / decay_tile_c(c); }
 // the gradients' passes have their roles exchanged: one launch serves all three if both head sizes have the same tiles
@@ -285,15 +286,16 @@ DecaySplit decay_split(int n, int T, int H, int dk, int dv, int dtype, bool back
     };
     DecaySplit best{1, DECAY_CHUNK * (chunks > 0 ? chunks : 1)};
     double least = INFINITY;
-    for (int want = 1; want <= chunks && (want == 1 || rows * want <= 16 * kNumCU); want += want < 4 ? 1 : want / 4) {
+    for (int want = 1; want <= chunks && (want == 1 || rows * want <= 16 * kNumCU); want += want < 32 ? 1 : want / 8) {
         const int per = (chunks + want - 1) / want, nseg = (chunks + per - 1) / per;
         double cost;
         if (!backward) cost = launch_cost(dk, rows * nseg * col_tiles(dv));
         else if (decay_one_launch(dk, dv)) cost = launch_cost(dk, rows * nseg * col_tiles(dv) * 3);
         else cost = launch_cost(dv, rows * nseg * col_tiles(dk) * 2) + launch_cost(dk, rows * nseg * col_tiles(dv));
-        if (nseg > 1) cost += 0.4 * launch_cost(dk, rows * (nseg - 1) * col_tiles(dv) * (backward ? 2 : 1)) + 10.0 / per;
-        if (cost * per < 0.99 * least) {
-            least = cost * per;
+        if (nseg > 1) cost += 0.4 * launch_cost(dk, rows * (nseg - 1) * col_tiles(dv) * (backward ? 2 : 1));
+        cost = cost * (per + 0.5) + (nseg > 1 ? 5.0 + 0.15 * nseg : 0.0);
+        if (cost < 0.99 * least) {
+            least = cost;
             best = DecaySplit{nseg, per * DECAY_CHUNK};
         }
     }
