@@ -1,0 +1,54 @@
+"""Temporal operators on inputs whose sums are exact in fp32 in any order: the result is then the oracle's, to the last bit of its type."""
+import pytest
+import torch
+
+from oracle import temporal as ot
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+TINY = 2.0 ** -22                   # of 1 + 2^-10 + 2^-22: in the last of its 24 bits, behind the 17 that two bf16 values hold
+DIMS = [(32, 32), (64, 64), (128, 128), (128, 32), (40, 72), (33, 65)]
+
+
+def _same_as_oracle(dtype, q, k, v, state, log_decay=None):
+    """A call with gradients (of the last token's first value: sums of one term) and the oracle's: every result the same numbers."""
+    from evfly_amd.temporal import decay_attention
+    ld = torch.zeros(q.shape[2]) if log_decay is None else log_decay
+    lc = [t.to(dtype).cuda().requires_grad_() for t in (q, k, v)] + [state.cuda().requires_grad_()]
+    lo = [t.double().requires_grad_() for t in (q, k, v, state)]
+    up = torch.zeros(*q.shape[:3], v.shape[-1])
+    up[:, -1, :, 0] = 1.0
+    out, new = decay_attention(*lc[:3], ld.cuda(), state=lc[3], scale=1.0)
+    want, wnew = ot.decay_attention(*lo[:3], ld, lo[3], scale=1.0)
+    got = [out, new, *torch.autograd.grad(out, lc, up.to(dtype).cuda())]
+    ref = [want, wnew, *torch.autograd.grad(want, lo, up.double())]
+    for name, a, b in zip(("out", "new_state", "dq", "dk", "dv", "dstate"), got, ref):
+        like = F32 if "state" in name else dtype
+        assert a.dtype == like
+        assert torch.equal(a.detach().cpu(), b.detach().to(like)), name
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("dk,dv", DIMS, ids=lambda d: str(d))
+@pytest.mark.parametrize("T", [3, 20, 64, 100])
+def test_state_enters_the_products_with_all_its_bits(gpu_device, T, dk, dv, dtype):
+    """q_t (S[0] - S[1]) = 2^-22 where S[0] = 1 + 2^-10 + 2^-22 and S[1] = 1 + 2^-10: what is left of the state's last bits is the whole result."""
+    q, k, v, S = torch.zeros(2, T, 2, dk), torch.zeros(2, T, 1, dk), torch.zeros(2, T, 1, dv), torch.zeros(2, 2, dk, dv)
+    q[..., 0], q[..., 1] = 1.0, -1.0
+    S[..., 0, :], S[..., 1, :] = 1 + 2.0 ** -10 + TINY, 1 + 2.0 ** -10
+    out = _same_as_oracle(dtype, q, k, v, S)
+    assert (out.float() == TINY).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("dk,dv", DIMS, ids=lambda d: str(d))
+@pytest.mark.parametrize("T", [3, 20, 64, 100])
+def test_pair_products_enter_the_sum_with_all_their_bits(gpu_device, T, dk, dv, dtype):
+    """Token 0 brings (1 + 2^-10 + 2^-22) v, token 1 -(1 + 2^-10) v: 2^-22 v is left from there on."""
+    q, k, v, S = torch.zeros(2, T, 2, dk), torch.zeros(2, T, 1, dk), torch.zeros(2, T, 1, dv), torch.zeros(2, 2, dk, dv)
+    q[..., 0], q[..., 1], q[..., 2] = 1.0, 2.0 ** -10, TINY
+    k[:, 0, :, :3], k[:, 1, :, :2] = 1.0, 1.0
+    v[:, 0], v[:, 1] = 1.0, -1.0
+    out = _same_as_oracle(dtype, q, k, v, S)
+    assert (out[:, 1:].float() == TINY).all()
