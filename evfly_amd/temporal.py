@@ -61,7 +61,7 @@ def _decay_fits(q, k, v, log_decay, state, lengths, lead):
     try:
         dt, dev, qs, ks, vs = q.dtype, q.device, q.shape, k.shape, v.shape
         H, KV, dk, dv = qs[-2], ks[-2], qs[-1], vs[-1]
-        return (len(qs) == lead + 2 and dt in _DTYPE and k.dtype is dt and v.dtype is dt and dev.type == "cuda" and k.device == dev and v.device == dev and
+        return (len(qs) == len(ks) == len(vs) == lead + 2 and dt in _DTYPE and k.dtype is dt and v.dtype is dt and dev.type == "cuda" and k.device == dev and v.device == dev and
                 ks[:lead] == qs[:lead] and vs[:lead] == qs[:lead] and ks[-1] == dk and vs[-2] == KV and KV > 0 and H > 0 and H % KV == 0 and
                 0 < dk <= MAX_HEAD_DIM and 0 < dv <= MAX_HEAD_DIM and
                 log_decay.dtype is torch.float32 and log_decay.shape == (H,) and log_decay.device == dev and not log_decay.requires_grad and
@@ -171,7 +171,7 @@ def _decay_backward(q, k, v, log_decay, state, lengths, scale, d_out, d_state, w
 
 
 def _new_state(q, v):
-    return torch.empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+    return torch.empty((q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=q.device)
 
 
 def _no_second_order(who):

@@ -1,0 +1,23 @@
+"""Calls of the temporal operators' public entries that are refused, and rarely made ones that are not."""
+import pytest
+import torch
+
+from _temporal import decay_inputs
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _cuda(d):
+    return {k: t.cuda() if isinstance(t, torch.Tensor) else t for k, t in d.items()}
+
+
+def test_k_and_v_of_another_rank_are_refused(gpu_device):
+    from evfly_amd.temporal import decay_attention, decay_attention_step
+    z = lambda *s: torch.zeros(*s, device="cuda")
+    for q, k, v in ((z(4, 8, 32), z(4, 32), z(4, 32)), (z(4, 8, 32), z(4, 2, 8, 32), z(4, 2, 8, 32)), (z(4, 8, 32), z(4, 8, 32), z(4, 2, 8, 32))):
+        with pytest.raises(ValueError):
+            decay_attention_step(q, k, v, z(8), z(4, 8, 32, 32))
+    for q, k, v in ((z(2, 100, 8, 64), z(2, 100, 2, 8, 64), z(2, 100, 2, 8, 64)), (z(2, 4, 4, 64), z(2, 4, 64), z(2, 4, 4, 64)), (z(2, 4, 4, 64), z(2, 4, 4, 64), z(2, 4, 64))):
+        with pytest.raises(ValueError):
+            decay_attention(q, k, v, z(q.shape[2]))
