@@ -13,6 +13,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -37,6 +38,19 @@ def _dense(t):
 
 def _workspace(nbytes, like):
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes > 0 else None
+
+
+def _refuse_unseen(who, tensors, recorded):
+    """The library's work is no torch operation: forward-mode differentiation takes its results for constants, a tracer for memory that nothing writes. (recorded: the
+    call is an autograd function's, which torch.jit.trace keeps as a whole.)"""
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who} has no forward-mode derivatives")
+    if not recorded and torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{who}: torch.jit.trace does not see its work")
+    if torch._C._len_torch_dispatch_stack() > 0:
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if get_proxy_mode() is not None:
+            raise RuntimeError(f"{who}: make_fx does not see its work")
 
 
 def _check_tokens(who, named, like):
@@ -207,7 +221,9 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     lengths (streams,) int32: tokens of each stream that are there, None = all; the others are not read, `out` is zero there.
     scale: dk ** -0.5 if None. Returns (out (streams, tokens, heads, dv), new state). Gradients to q, k, v and state."""
     scale = _check_decay("decay_attention", q, k, v, log_decay, state, lengths, scale, 2)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
+    recorded = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad))
+    _refuse_unseen("decay_attention", (q, k, v, log_decay, state), recorded)
+    if recorded:
         return _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale)
     new_state = _new_state(q, v)
     return _decay_forward(q, k, v, log_decay, state, lengths, scale, new_state), new_state
@@ -230,6 +246,7 @@ def decay_attention_step(q, k, v, log_decay, state, lengths=None, scale=None, ne
         dst = new_state
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or dst.requires_grad):
         raise ValueError(f"{who} has no gradients: call decay_attention, or wrap the call in torch.no_grad()")
+    _refuse_unseen(who, (q, k, v, log_decay, state, new_state), False)
     out = _decay_forward(q, k, v, log_decay, state, lengths, scale, dst)
     if not dst.is_inference():                                   # (an inference tensor has no version)
         torch.autograd.graph.increment_version(dst)              # written behind autograd's back
@@ -372,9 +389,15 @@ def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None,
     if gate is not None:
         rows_per_gate, gate_f32 = max(1, _gate_rows(f, gate)), int(gate.dtype is torch.float32)
     opt = (rows_per_gate, gate_f32, _GATE_ACT[gate_act], _NORM[post], _NORM[pre], eps)
+    ins = (f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias)
+    recorded = False
     if torch.is_grad_enabled():
-        for t in (f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias):
+        for t in ins:
             if t is not None and t.requires_grad:
-                got = _BlockNorm.apply(f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias, opt)
-                return got if isinstance(got, tuple) else (got, None)
-    return _block_forward(f, x, gate, res_scale, post_weight, post_bias, pre_weight, pre_bias, opt)
+                recorded = True
+                break
+    _refuse_unseen("block_norm", ins, recorded)
+    if recorded:
+        got = _BlockNorm.apply(*ins, opt)
+        return got if isinstance(got, tuple) else (got, None)
+    return _block_forward(*ins, opt)

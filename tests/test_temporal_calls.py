@@ -50,3 +50,64 @@ def test_k_and_v_of_another_rank_are_refused():
         for q, k, v in bad:
             with pytest.raises(ValueError, match="must be a tensor"):
                 temporal._refuse_decay("decay_attention", q, k, v, z(8), None, None, lead)
+
+
+# ---- what torch does not see of the library's work
+@pytest.fixture
+def no_device(monkeypatch):
+    """The entries on CPU tensors: every argument fits, the library's calls do nothing."""
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *a: 0
+    monkeypatch.setattr(temporal._lib, "lib", lambda: None)
+    monkeypatch.setattr(temporal._lib, "load_library", Nothing)
+    monkeypatch.setattr(temporal, "_decay_fits", lambda *a: True)
+    monkeypatch.setattr(temporal, "_block_fits", lambda *a: True)
+    monkeypatch.setattr(temporal, "_getDevice", lambda: -1)
+    monkeypatch.setattr(temporal, "_rawStream", lambda i: 0)
+
+
+Q, LD, S = torch.zeros(1, 3, 2, 4), torch.zeros(2), torch.zeros(1, 2, 4, 4)
+ENTRIES = {"decay_attention": lambda x: temporal.decay_attention(x, Q, Q, LD, state=S)[0],
+           "decay_attention_step": lambda x: temporal.decay_attention_step(x[:, 0], Q[:, 0], Q[:, 0], LD, S.clone()),
+           "block_norm": lambda x: temporal.block_norm(x, Q, pre="rms")[1]}
+OF_OTHERS = {"v": (Q, lambda t: temporal.decay_attention(Q, Q, t, LD)), "log_decay": (LD, lambda t: temporal.decay_attention(Q, Q, Q, t)),
+             "state": (S, lambda t: temporal.decay_attention(Q, Q, Q, LD, state=t)), "step_state": (S, lambda t: temporal.decay_attention_step(Q[:, 0], Q[:, 0], Q[:, 0], LD, t)),
+             "x": (Q, lambda t: temporal.block_norm(Q, t)), "gate": (torch.zeros(4), lambda t: temporal.block_norm(Q, gate=t)),
+             "weight": (torch.zeros(4), lambda t: temporal.block_norm(Q, pre="rms", pre_weight=t))}
+
+
+@pytest.mark.parametrize("name", list(ENTRIES))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(no_device, name, grad):
+    call = ENTRIES[name]
+    with torch.autograd.forward_ad.dual_level():
+        x = Q.clone().requires_grad_(grad and name != "decay_attention_step")
+        with pytest.raises(NotImplementedError):
+            call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(Q)))
+        assert call(Q).shape[-1] == 4                                # a level alone is nothing to refuse
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(call, (Q,), (torch.ones_like(Q),))
+
+
+@pytest.mark.parametrize("name", list(OF_OTHERS))
+def test_forward_mode_of_the_other_arguments_is_refused(no_device, name):
+    t, call = OF_OTHERS[name]
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        call(torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t)))
+
+
+@pytest.mark.parametrize("name", list(ENTRIES))
+def test_tracers_are_refused(no_device, name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call = ENTRIES[name]
+    with pytest.raises(RuntimeError, match="does not see"):
+        torch.jit.trace(call, (Q,), check_trace=False)
+    with pytest.raises(RuntimeError, match="does not see"):
+        make_fx(call)(Q)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(call)(torch.stack([Q, Q]))
+    if name != "decay_attention_step":
+        with pytest.raises(RuntimeError, match="does not see"):
+            make_fx(lambda x: call(x.requires_grad_()))(Q.clone())
+    assert call(Q).shape[-1] == 4
