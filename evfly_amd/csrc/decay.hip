@@ -192,6 +192,12 @@ bool recurrent(int tokens, int dk, int dv, int dtype) {
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// a buffer of states that shares some of its bytes with another one: a block would write what another still reads
+bool overlaps(const float *a, const float *b, int64_t floats) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && (x < y ? y - x : x - y) < (uintptr_t)floats * 4;
+}
+
 struct Tokens {              // one token tensor: pointer, element strides, heads of the pass per head of it, width
     const void *p;
     int64_t s[3];
@@ -322,6 +328,8 @@ extern "C" int evfly_decay_attention_forward(const void *q, const void *k, const
     const Ws ws = decay_ws(n_streams, tokens, heads, kv_heads, dk, dv, dtype, false);
     EVFLY_REQUIRE(workspace_bytes >= ws.bytes && (ws.bytes == 0 || (workspace && aligned16(workspace))),
                   "decay_attention_forward: workspace smaller than evfly_decay_attention_workspace_bytes, or not 16-byte aligned");
+    EVFLY_REQUIRE(state_in == state_out || !overlaps(state_in, state_out, (int64_t)n_streams * heads * dk * dv),
+                  "decay_attention_forward: state_in and state_out overlap in part");
     hipStream_t st = as_stream(stream);
     const int rep = heads / kv_heads;
     Tokens tq{q, {}, 1, dk}, tk{k, {}, rep, dk}, tv{v, {}, rep, dv};

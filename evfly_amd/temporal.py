@@ -243,6 +243,8 @@ def decay_attention_step(q, k, v, log_decay, state, lengths=None, scale=None, ne
         _check_f32(who, "new_state", new_state, state.shape, q.device)
         if not new_state.is_contiguous():
             raise ValueError(f"{who}: new_state must be a contiguous tensor")
+        if 0 < abs(new_state.data_ptr() - state.data_ptr()) < 4 * state.numel():
+            raise ValueError(f"{who}: state and new_state overlap in part")
         dst = new_state
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or dst.requires_grad):
         raise ValueError(f"{who} has no gradients: call decay_attention, or wrap the call in torch.no_grad()")

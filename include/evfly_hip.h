@@ -353,7 +353,8 @@ int evfly_model_profile_reset(evfly_model *m);
  * k, then of v; the last dimension is contiguous), NULL = contiguous tensors; out is contiguous.
  * log_decay (heads) fp32: 0 keeps everything, -inf keeps nothing (out_t = scale * (q_t . k_t) v_t); positive values grow and are
  * computed as they stand.
- * state_in (n_streams, heads, dk, dv) fp32 or NULL = zeros; state_out the same, or NULL = not wanted; they may be the same buffer.
+ * state_in (n_streams, heads, dk, dv) fp32 or NULL = zeros; state_out the same, or NULL = not wanted; they may be the same buffer, but not
+ * overlap in part. No other output shares memory with an input or with another output.
  * lengths (n_streams) int32 or NULL: stream i has lengths[i] tokens (taken into [0, tokens]); what q, k, v hold behind them is
  * not read, out is zero there, and state_out is the state after the stream's last token (a stream of no tokens keeps its state).
  * Inside a sequence a non-finite k or v reaches every later token, and may reach the earlier tokens of its own group of 64.

@@ -21,3 +21,18 @@ def test_k_and_v_of_another_rank_are_refused(gpu_device):
     for q, k, v in ((z(2, 100, 8, 64), z(2, 100, 2, 8, 64), z(2, 100, 2, 8, 64)), (z(2, 4, 4, 64), z(2, 4, 64), z(2, 4, 4, 64)), (z(2, 4, 4, 64), z(2, 4, 4, 64), z(2, 4, 64))):
         with pytest.raises(ValueError):
             decay_attention(q, k, v, z(q.shape[2]))
+
+
+def test_states_that_overlap_in_part_are_refused(gpu_device):
+    """Shifted views of one buffer are refused; neighbouring ones and the same one are not."""
+    from evfly_amd.temporal import decay_attention_step
+    d = _cuda(decay_inputs(4, 1, 2, 2, 32, 32, F32, seed=30))
+    q, k, v = (d[m][:, 0] for m in "qkv")
+    buf = torch.zeros(9, 2, 32, 32, device="cuda")
+    buf[:4] = d["state"]
+    for a, b in ((buf[:4], buf[1:5]), (buf[1:5], buf[:4])):
+        with pytest.raises(ValueError, match="overlap"):
+            decay_attention_step(q, k, v, d["log_decay"], a, new_state=b)
+    out = decay_attention_step(q, k, v, d["log_decay"], buf[:4], new_state=buf[4:8])
+    assert torch.equal(buf[:4], d["state"]) and not buf[8].any()
+    assert torch.equal(decay_attention_step(q, k, v, d["log_decay"], d["state"]), out) and torch.equal(d["state"], buf[4:8])

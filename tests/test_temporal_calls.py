@@ -111,3 +111,31 @@ def test_tracers_are_refused(no_device, name):
         with pytest.raises(RuntimeError, match="does not see"):
             make_fx(lambda x: call(x.requires_grad_()))(Q.clone())
     assert call(Q).shape[-1] == 4
+
+
+# ---- state buffers that share memory
+def _c_call(name, good, **bad):
+    from evfly_amd import _lib
+    L = _lib.load_library()
+    assert getattr(L, name)(*{**good, **bad}.values()) == -1
+    return L.evfly_last_error().decode()
+
+
+def test_states_that_overlap_in_part_are_refused(no_device):
+    buf = torch.zeros(5, 2, 4, 4)
+    q = torch.zeros(4, 2, 4)
+    for state, new in ((buf[:-1], buf[1:]), (buf[1:], buf[:-1]), (buf.view(-1)[:128].view(4, 2, 4, 4), buf.view(-1)[1:129].view(4, 2, 4, 4))):
+        with pytest.raises(ValueError, match="overlap"):
+            temporal.decay_attention_step(q, q, q, LD, state, new_state=new)
+    whole = torch.zeros(8, 2, 4, 4)
+    for state, new in ((whole[:4], whole[4:]), (whole[4:], whole[:4]), (whole[:4], whole[:4])):
+        temporal.decay_attention_step(q, q, q, LD, state, new_state=new)
+
+
+def test_states_that_overlap_in_part_are_refused_by_the_abi():
+    from test_temporal import DECAY, X
+    size = 4 * 32 * 32 * 4
+    for off in (4, 4096, size - 4):
+        for a, b in ((X, X + off), (X + off, X)):
+            for T in (1, 64, 200):
+                assert "overlap" in _c_call("evfly_decay_attention_forward", DECAY, T=T, state_in=a, state_out=b, ws=X, ws_bytes=1 << 40)
