@@ -376,7 +376,9 @@ extern "C" int evfly_decay_attention_backward(const void *q, const void *k, cons
     token_strides(strides_host ? strides_host + 3 : nullptr, tokens, kv_heads, dk, tk.s);
     token_strides(strides_host ? strides_host + 6 : nullptr, tokens, kv_heads, dv, tv.s);
     token_strides(nullptr, tokens, heads, dv, to.s);
-    EVFLY_REQUIRE(!d_state_in || d_state_in != d_state_out, "decay_attention_backward: d_state_in is d_state_out");
+    const int64_t states = (int64_t)n_streams * heads * dk * dv;
+    EVFLY_REQUIRE(!overlaps(d_state_in, state_in, states) && !overlaps(d_state_in, d_state_out, states),
+                  "decay_attention_backward: d_state_in shares memory with state_in or d_state_out");
     Run run{dtype, st, DecayPass{}};
     const DecaySplit sp = decay_split(n_streams, tokens, heads, dk, dv, dtype, true);
     char *const w = static_cast<char *>(workspace);

@@ -371,8 +371,8 @@ int evfly_decay_attention_forward(const void *q, const void *k, const void *v, c
                                   int tokens, int heads, int kv_heads, int dk, int dv, float scale, int dtype, void *out,
                                   float *state_out, void *workspace, int64_t workspace_bytes, void *stream);
 /* Its gradients: d_out (n_streams, tokens, heads, dv) and d_state_out (n_streams, heads, dk, dv) fp32 or NULL = zeros come in;
- * dq, dk, dv (contiguous, shaped like q, k, v; the sum over the query heads that share a key / value head) and d_state_in (fp32, may be NULL,
- * not the buffer of d_state_out) go out. d_out is not read and dq, dk, dv are zero behind a stream's length. log_decay is a constant: it has no gradient. */
+ * dq, dk, dv (contiguous, shaped like q, k, v; the sum over the query heads that share a key / value head) and d_state_in (fp32, may be NULL;
+ * no memory of state_in's or d_state_out's, which other blocks still read) go out. d_out is not read and dq, dk, dv are zero behind a stream's length. log_decay is a constant: it has no gradient. */
 int evfly_decay_attention_backward(const void *q, const void *k, const void *v, const int64_t *strides_host,
                                    const float *log_decay, const float *state_in, const int32_t *lengths, const void *d_out,
                                    const float *d_state_out, int n_streams, int tokens, int heads, int kv_heads, int dk, int dv,

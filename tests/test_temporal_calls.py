@@ -139,3 +139,15 @@ def test_states_that_overlap_in_part_are_refused_by_the_abi():
         for a, b in ((X, X + off), (X + off, X)):
             for T in (1, 64, 200):
                 assert "overlap" in _c_call("evfly_decay_attention_forward", DECAY, T=T, state_in=a, state_out=b, ws=X, ws_bytes=1 << 40)
+
+
+def test_the_states_gradient_has_a_buffer_of_its_own():
+    """The pass that forms dq reads the state while the one that forms dv writes its gradient."""
+    from test_temporal import DECAY_BACK, X
+    size = 4 * 32 * 32 * 4
+    for other in ("state_in", "d_state"):
+        for off in (0, 4, size - 4):
+            for a, b in ((X, X + off), (X + off, X)):
+                for T in (1, 64, 2000):
+                    said = _c_call("evfly_decay_attention_backward", DECAY_BACK, T=T, ws=X, ws_bytes=1 << 40, ds=a, **{other: b})
+                    assert "d_state_in" in said and "memory" in said
