@@ -52,3 +52,16 @@ def test_pair_products_enter_the_sum_with_all_their_bits(gpu_device, T, dk, dv, 
     v[:, 0], v[:, 1] = 1.0, -1.0
     out = _same_as_oracle(dtype, q, k, v, S)
     assert (out[:, 1:].float() == TINY).all()
+
+
+@pytest.mark.parametrize("dk,dv", DIMS, ids=lambda d: str(d))
+@pytest.mark.parametrize("T", [64, 128, 1024])
+def test_a_chunk_is_added_to_the_state_whole(gpu_device, T, dk, dv):
+    """fp32: every chunk of 64 tokens adds 64 / 16 = 4 to a state of 2^24, whose neighbours are 2 apart: 4 is there, a token's 1/16 alone would not be. The same
+    backwards for the state's gradient."""
+    from evfly_amd.temporal import decay_attention
+    q, k, v = (torch.full((2, T, h, d), x, device="cuda", requires_grad=True) for h, d, x in ((2, dk, 0.0625), (1, dk, 0.0625), (1, dv, 1.0)))
+    S = torch.full((2, 2, dk, dv), 2.0 ** 24, device="cuda", requires_grad=True)
+    out, new = decay_attention(q, k, v, torch.zeros(2, device="cuda"), state=S, scale=1.0)
+    assert (new == 2.0 ** 24 + T // 16).all()
+    assert (torch.autograd.grad([out, new], S, [torch.ones_like(out), torch.full_like(new, 2.0 ** 24)])[0] == 2.0 ** 24 + T // 16).all()
