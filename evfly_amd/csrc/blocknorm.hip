@@ -181,7 +181,10 @@ template <typename T, int G> __device__ __forceinline__ float normalise(float (&
         q[0] = fmaf(v[j], v[j], q[0]);
     }
     row_sum<G>(q, red, turn);
-    const float r = __builtin_amdgcn_rsqf(fmaf(q[0], inv_c, eps));
+    // (the instruction takes a subnormal for zero: such a mean square is brought into the normal numbers and its root back)
+    const float ms = fmaf(q[0], inv_c, eps);
+    const bool tiny = ms < 0x1p-126f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? ms * 0x1p32f : ms) * (tiny ? 0x1p16f : 1.f);
 #pragma unroll
     for (int j = 0; j < E; ++j) v[j] *= r;
     return r;

@@ -65,3 +65,23 @@ def test_a_chunk_is_added_to_the_state_whole(gpu_device, T, dk, dv):
     out, new = decay_attention(q, k, v, torch.zeros(2, device="cuda"), state=S, scale=1.0)
     assert (new == 2.0 ** 24 + T // 16).all()
     assert (torch.autograd.grad([out, new], S, [torch.ones_like(out), torch.full_like(new, 2.0 ** 24)])[0] == 2.0 ** 24 + T // 16).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("C", [32, 256, 2048])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -132])
+def test_block_norm_of_rows_whose_mean_square_is_subnormal(gpu_device, eps, kind, C, dtype):
+    """+-2^-66: squares 2^-132, which fp32 holds below its normal numbers, so does their mean. eps 0: +-1 back, within the reciprocal root's ulp, the output's
+    product and its half step; eps = 2^-132: sqrt(1/2) of it."""
+    from evfly_amd.temporal import block_norm
+    f = torch.full((5, C), 2.0 ** -66)
+    f[:, 1::2] *= -1
+    f[3] = 2.0 ** -60 * f[3].sign()                                          # (and one that is not: 2^-120)
+    f = f.to(dtype)
+    want = f.double() / torch.sqrt(f.double().square().mean(-1, keepdim=True) + eps)
+    lv = f.cuda().requires_grad_()
+    tol = 4 * 2.0 ** -24 + torch.finfo(dtype).eps / 2
+    for got in (block_norm(lv, pre=kind, eps=eps)[1], block_norm(lv, post=kind, eps=eps)[0]):
+        assert ((got.detach().double().cpu() - want).abs() <= tol * want.abs()).all()
+        assert torch.isfinite(torch.autograd.grad(got[:, 0].sum(), lv)[0]).all()
