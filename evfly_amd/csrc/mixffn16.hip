@@ -14,7 +14,7 @@
 //      channels, block-diagonal in the group (half of A is zero: 512 useful flop per cycle and SIMD, twice the 4x4x4 MFMAs
 //      gconv.hip uses, and no register window: 20 weight registers per lane instead of 72); B = one 16-B unit of the tile per lane and
 //      MFMA, straight from LDS: five MFMAs per task. D[channel][token] leaves a lane with four adjacent channels of one token: GELU
-//      (two values per v_pk_*_f32, the previous task's under this task's LDS reads), one rounding, 8 B into the hidden tile.
+//      (the previous task's under this task's LDS reads), one rounding, 8 B into the hidden tile.
 //   C. mlp2's partial sums over the slab's 32 hidden channels: D[out channel][token] += W2[:, slab] x tile, accumulated in
 //      registers across all slabs (C / 32 accumulator tiles per wave).
 // Every LDS tile is a set of 16-B-unit PLANES ([unit][row]: a row = token, pixel or weight row): the 16 / 32 lanes of a read phase
@@ -92,62 +92,52 @@ __device__ __forceinline__ mf_i32x4 mf_srd(const void *p, unsigned bytes) {
     return s;
 }
 
-// packed fp32 arithmetic: one v_pk_* costs the SIMD what one scalar-lane op does (tools/ubench/mfma_valu.hip). Inline asm: hipcc
-// scalarises packed IR whose results are read element-wise. Constants come as SGPR pairs (one constant-bus operand per instruction).
-__device__ __forceinline__ mf_f32x2 pk_mul(mf_f32x2 a, mf_f32x2 b) { mf_f32x2 d; asm("v_pk_mul_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b)); return d; }
-__device__ __forceinline__ mf_f32x2 pk_fma_s(mf_f32x2 a, mf_f32x2 b, mf_f32x2 c) { mf_f32x2 d; asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c)); return d; }
-__device__ __forceinline__ mf_f32x2 pk_fma_ss(mf_f32x2 a, mf_f32x2 s, mf_f32x2 c) { mf_f32x2 d; asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "s"(s), "v"(c)); return d; }
+// two values side by side, each an instruction of its own (packed fp32 instructions are kept out of this library: Makefile)
+__device__ __forceinline__ mf_f32x2 mul2(mf_f32x2 a, mf_f32x2 b) { return mf_f32x2{a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ mf_f32x2 fma2(mf_f32x2 a, mf_f32x2 b, mf_f32x2 c) { return mf_f32x2{fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
 
 // erf-GELU of two values. erf(v) = v P(v^2) / Q(v^2) on |v| <= 3.5 with cubic P and Q (minimax fit, tools/mixffn_check.py MF_GELU=1:
 // |error| <= 1.3e-5 against erf, <= 7e-5 on the GELU -- two orders below the bf16 rounding of the result; gconv.hip's sixth / fourth
-// degree form (4.5e-7) costs four more packed FMAs per pair, and this phase is VALU-bound), Horner steps packed
+// degree form (4.5e-7) costs four more FMAs a value, and this phase is VALU-bound)
 #define MF_C2(x) (mf_f32x2{(x), (x)})
 #ifndef EVFLY_MF_GELU_POLY
 #define EVFLY_MF_GELU_POLY 1
 #endif
 #if EVFLY_MF_GELU_POLY
-// Round 5: erf(v) = v P(v^2) on |v| <= 3 with a seventh-degree P and P(9) 3 pinned to 1 (beyond the clamp the GELU is exactly a or 0;
+// erf(v) = v P(v^2) on |v| <= 3 with a seventh-degree P and P(9) 3 pinned to 1 (beyond the clamp the GELU is exactly a or 0;
 // fit with its error weighted by the GELU's sensitivity 0.5 |a|, tools/mixffn_check.py MF_GELU=2: |error| <= 9.6e-5 on the GELU in
-// fp32 Horner arithmetic, the rational form's 7e-5 class, 40 times below the bf16 rounding of the result) -- seven packed FMAs and NO
+// fp32 Horner arithmetic, the rational form's 7e-5 class, 40 times below the bf16 rounding of the result) -- seven FMAs and NO
 // reciprocal: the two v_rcp_f32 of the rational form are transcendental-rate instructions in a VALU-bound phase.
 __device__ __forceinline__ mf_f32x2 mf_gelu2(mf_f32x2 a) {
-    mf_f32x2 v;      // (first reader of `a` is compiler-visible: see the rational form below)
+    mf_f32x2 v;
     v[0] = __builtin_amdgcn_fmed3f(a[0] * 0.70710678118654752440f, -3.0f, 3.0f);
     v[1] = __builtin_amdgcn_fmed3f(a[1] * 0.70710678118654752440f, -3.0f, 3.0f);
-    const mf_f32x2 v2 = pk_mul(v, v);
-    mf_f32x2 p = pk_fma_ss(v2, MF_C2(-3.09380368435086e-07f), MF_C2(1.3807954019284807e-05f));
-    p = pk_fma_s(p, v2, MF_C2(-0.00026738294400274754f));
-    p = pk_fma_s(p, v2, MF_C2(0.0029750755056738853f));
-    p = pk_fma_s(p, v2, MF_C2(-0.021316345781087875f));
-    p = pk_fma_s(p, v2, MF_C2(0.10481300950050354f));
-    p = pk_fma_s(p, v2, MF_C2(-0.3703286349773407f));
-    p = pk_fma_s(p, v2, MF_C2(1.1269229650497437f));
-    const mf_f32x2 e = pk_mul(v, p);
-    return pk_mul(a, pk_fma_ss(e, MF_C2(0.5f), MF_C2(0.5f)));      // 0.5 a (1 + erf)
+    const mf_f32x2 v2 = mul2(v, v);
+    mf_f32x2 p = fma2(v2, MF_C2(-3.09380368435086e-07f), MF_C2(1.3807954019284807e-05f));
+    p = fma2(p, v2, MF_C2(-0.00026738294400274754f));
+    p = fma2(p, v2, MF_C2(0.0029750755056738853f));
+    p = fma2(p, v2, MF_C2(-0.021316345781087875f));
+    p = fma2(p, v2, MF_C2(0.10481300950050354f));
+    p = fma2(p, v2, MF_C2(-0.3703286349773407f));
+    p = fma2(p, v2, MF_C2(1.1269229650497437f));
+    const mf_f32x2 e = mul2(v, p);
+    return mul2(a, fma2(e, MF_C2(0.5f), MF_C2(0.5f)));      // 0.5 a (1 + erf)
 }
 #else
 __device__ __forceinline__ mf_f32x2 mf_gelu2(mf_f32x2 a) {
-    // (the first reader of `a` is compiler-visible code: the caller's `a` comes out of an MFMA, and hipcc's hazard recogniser puts
-    // the wait states between the matrix pipe's write and a VALU read only in front of instructions it can see -- an inline-asm
-    // consumer right behind the last MFMA of a task read the registers early)
     mf_f32x2 v;
     v[0] = __builtin_amdgcn_fmed3f(a[0] * 0.70710678118654752440f, -3.5f, 3.5f);
     v[1] = __builtin_amdgcn_fmed3f(a[1] * 0.70710678118654752440f, -3.5f, 3.5f);
-    const mf_f32x2 v2 = pk_mul(v, v);
-    mf_f32x2 p = pk_fma_ss(v2, MF_C2(0.0007302758749574423f), MF_C2(0.04286076873540878f));
-    p = pk_fma_s(p, v2, MF_C2(0.15528972446918488f));
-    p = pk_fma_s(p, v2, MF_C2(1.1283745765686035f));
-    mf_f32x2 q = pk_fma_ss(v2, MF_C2(0.009142078459262848f), MF_C2(0.09490722417831421f));
-    q = pk_fma_s(q, v2, MF_C2(0.470951646566391f));
-    q = pk_fma_s(q, v2, MF_C2(1.0f));
-    // (the reciprocals from inside the asm, with the wait state gfx950 wants between a transcendental result and the VALU
-    // instruction that reads it: hipcc's hazard recogniser does not look into the inline-asm consumer and left none -- the
-    // second element of every pair came out wrong)
-    float r0, r1;
-    asm("v_rcp_f32 %0, %2\n\tv_rcp_f32 %1, %3\n\ts_nop 1" : "=&v"(r0), "=&v"(r1) : "v"(q[0]), "v"(q[1]));
-    const mf_f32x2 r = {r0, r1};
-    const mf_f32x2 e = pk_mul(pk_mul(v, p), r);
-    return pk_mul(a, pk_fma_ss(e, MF_C2(0.5f), MF_C2(0.5f)));      // 0.5 a (1 + erf)
+    const mf_f32x2 v2 = mul2(v, v);
+    mf_f32x2 p = fma2(v2, MF_C2(0.0007302758749574423f), MF_C2(0.04286076873540878f));
+    p = fma2(p, v2, MF_C2(0.15528972446918488f));
+    p = fma2(p, v2, MF_C2(1.1283745765686035f));
+    mf_f32x2 q = fma2(v2, MF_C2(0.009142078459262848f), MF_C2(0.09490722417831421f));
+    q = fma2(q, v2, MF_C2(0.470951646566391f));
+    q = fma2(q, v2, MF_C2(1.0f));
+    const mf_f32x2 r = {__builtin_amdgcn_rcpf(q[0]), __builtin_amdgcn_rcpf(q[1])};
+    const mf_f32x2 e = mul2(mul2(v, p), r);
+    return mul2(a, fma2(e, MF_C2(0.5f), MF_C2(0.5f)));      // 0.5 a (1 + erf)
 }
 #endif
 

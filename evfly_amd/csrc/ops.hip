@@ -528,11 +528,8 @@ __global__ __launch_bounds__(256) void k_grouped_conv_gelu(const float *__restri
 
 // LDS-tiled variant for small maps (H*W*32*4 B <= 64 KB; both ViT stages): one block = one frame x a slab of 32 channels
 // (4 groups). The slab is staged once; thread = (PAIR of adjacent output channels of one group, pixel lane): the two
-// channels read the same eight inputs per tap, so their 2 x 72 FMAs run as 72 v_pk_fma_f32 on the accumulator pair with
-// the input broadcast from one half of its register pair (op_sel) and the weight pair (w[co][k][t], w[co + 1][k][t]) in
-// registers -- a packed f32 op costs the SIMD what one v_fma_f32 does (tools/ubench/mfma_valu.hip). Inline asm: hipcc
-// scalarises packed IR whose results are read element-wise. Per output the operands and their order are those of the
-// untiled kernel (k fastest, then the taps): the same bits.
+// channels read the same eight inputs per tap, so an input read from LDS serves both; the weight pair (w[co][k][t], w[co + 1][k][t])
+// is in registers. Per output the operands and their order are those of the untiled kernel (k fastest, then the taps): the same bits.
 typedef float gc_f32x2 __attribute__((ext_vector_type(2)));
 typedef float gc_f32x4 __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void k_grouped_conv_gelu_lds(const float *__restrict__ x, int H, int W, int Ce,
@@ -568,14 +565,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
                 const gc_f32x4 v0 = sp[0], v1 = sp[1];
                 const gc_f32x2 i01 = v0.xy, i23 = v0.zw, i45 = v1.xy, i67 = v1.zw;
                 const int t = ky * 3 + kx;
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "+v"(acc) : "v"(i01), "v"(wp[0 * 9 + t]));
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "+v"(acc) : "v"(i01), "v"(wp[1 * 9 + t]));
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "+v"(acc) : "v"(i23), "v"(wp[2 * 9 + t]));
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "+v"(acc) : "v"(i23), "v"(wp[3 * 9 + t]));
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "+v"(acc) : "v"(i45), "v"(wp[4 * 9 + t]));
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "+v"(acc) : "v"(i45), "v"(wp[5 * 9 + t]));
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "+v"(acc) : "v"(i67), "v"(wp[6 * 9 + t]));
-                asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "+v"(acc) : "v"(i67), "v"(wp[7 * 9 + t]));
+                acc = {fmaf(i01.x, wp[0 * 9 + t].x, acc.x), fmaf(i01.x, wp[0 * 9 + t].y, acc.y)};
+                acc = {fmaf(i01.y, wp[1 * 9 + t].x, acc.x), fmaf(i01.y, wp[1 * 9 + t].y, acc.y)};
+                acc = {fmaf(i23.x, wp[2 * 9 + t].x, acc.x), fmaf(i23.x, wp[2 * 9 + t].y, acc.y)};
+                acc = {fmaf(i23.y, wp[3 * 9 + t].x, acc.x), fmaf(i23.y, wp[3 * 9 + t].y, acc.y)};
+                acc = {fmaf(i45.x, wp[4 * 9 + t].x, acc.x), fmaf(i45.x, wp[4 * 9 + t].y, acc.y)};
+                acc = {fmaf(i45.y, wp[5 * 9 + t].x, acc.x), fmaf(i45.y, wp[5 * 9 + t].y, acc.y)};
+                acc = {fmaf(i67.x, wp[6 * 9 + t].x, acc.x), fmaf(i67.x, wp[6 * 9 + t].y, acc.y)};
+                acc = {fmaf(i67.y, wp[7 * 9 + t].x, acc.x), fmaf(i67.y, wp[7 * 9 + t].y, acc.y)};
             }
         }
         float2 o;

@@ -185,10 +185,7 @@ __device__ __forceinline__ void produce_patch(const ConvDesc &d, const WinoGeom 
     // columns of each of the three rows are read once per run (four 8-B LDS reads), the nine weight vectors once per run, the
     // index arithmetic once per run -- per (pair, group) item they were two thirds of the producer's VALU instructions, and on
     // this layer the SIMD is VALU + MFMA bound (tools/wino_ts_pre.py: the producer was 46 % of a wave's life). The
-    // 72 * CIN FMAs per pair run as 36 * CIN v_pk_fma_f32 on register pairs (channels (0, 1) and (2, 3) of a pixel) with the
-    // frame value broadcast from one half of its pair (op_sel): a packed f32 op costs the SIMD what one v_fma_f32 does
-    // (tools/ubench/mfma_valu.hip). Inline asm: hipcc scalarises packed IR whose results are read element-wise. Same
-    // operands, same order (ky, kx, ci) per lane as k_e11: bitwise identical.
+    // accumulators are pairs of channels, (0, 1) and (2, 3) of a pixel. Same operands, same order (ky, kx, ci) per lane as k_e11: bitwise identical.
     const int ch = tid & 7, pairs_row = g.PW >> 1;
     const int nruns = g.IMGS * g.PH * g.rpr;
     for (int u = tid >> 3; u < ((kAbl & 2048) ? 0 : nruns); u += NTHR / 8) {        // (ablation 2048: no producer arithmetic)
@@ -215,18 +212,18 @@ __device__ __forceinline__ void produce_patch(const ConvDesc &d, const WinoGeom 
                         const int col = p6 + kx;
                         if (ky == 0 && ci == 0 && kx == 0) {      // first tap: accumulate from the bias (col = p6)
                             if (col & 1) {
-                                asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "=v"(al[p6]) : "v"(fp[col >> 1]), "v"(wl2), "v"(bl2));
-                                asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "=v"(ah[p6]) : "v"(fp[col >> 1]), "v"(wh2), "v"(bh2));
+                                al[p6] = {fmaf(fp[col >> 1].y, wl2.x, bl2.x), fmaf(fp[col >> 1].y, wl2.y, bl2.y)};
+                                ah[p6] = {fmaf(fp[col >> 1].y, wh2.x, bh2.x), fmaf(fp[col >> 1].y, wh2.y, bh2.y)};
                             } else {
-                                asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "=v"(al[p6]) : "v"(fp[col >> 1]), "v"(wl2), "v"(bl2));
-                                asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "=v"(ah[p6]) : "v"(fp[col >> 1]), "v"(wh2), "v"(bh2));
+                                al[p6] = {fmaf(fp[col >> 1].x, wl2.x, bl2.x), fmaf(fp[col >> 1].x, wl2.y, bl2.y)};
+                                ah[p6] = {fmaf(fp[col >> 1].x, wh2.x, bh2.x), fmaf(fp[col >> 1].x, wh2.y, bh2.y)};
                             }
                         } else if (col & 1) {
-                            asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "+v"(al[p6]) : "v"(fp[col >> 1]), "v"(wl2));
-                            asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "+v"(ah[p6]) : "v"(fp[col >> 1]), "v"(wh2));
+                            al[p6] = {fmaf(fp[col >> 1].y, wl2.x, al[p6].x), fmaf(fp[col >> 1].y, wl2.y, al[p6].y)};
+                            ah[p6] = {fmaf(fp[col >> 1].y, wh2.x, ah[p6].x), fmaf(fp[col >> 1].y, wh2.y, ah[p6].y)};
                         } else {
-                            asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "+v"(al[p6]) : "v"(fp[col >> 1]), "v"(wl2));
-                            asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "+v"(ah[p6]) : "v"(fp[col >> 1]), "v"(wh2));
+                            al[p6] = {fmaf(fp[col >> 1].x, wl2.x, al[p6].x), fmaf(fp[col >> 1].x, wl2.y, al[p6].y)};
+                            ah[p6] = {fmaf(fp[col >> 1].x, wh2.x, ah[p6].x), fmaf(fp[col >> 1].x, wh2.y, ah[p6].y)};
                         }
                     }
                 }
