@@ -228,7 +228,7 @@ __global__ __launch_bounds__(512) void k_clstm16_seq(const float *__restrict__ z
 // written by other CUs a moment ago, each is requested once per step, so the L1 has nothing to give and no buffer_inv is needed -- the
 // acquire cost 1.7 us per step plus a stalled vector-memory pipe behind it: -DEVFLY_CO_ACQ=1, C5 0.282 -> 0.256 ms per 16 steps).
 // Nothing depends on where a block runs; the b % 8 arithmetic below only keeps a group's traffic inside one XCD's L2 when the
-// dispatcher places blocks the way it has been observed to. Counters: one word per (group, step), zeroed by a memset node in front of
+// dispatcher places blocks the way it has been observed to. Counters: one word per (group, step), zeroed by a fill kernel in front of
 // every launch. Same fragment order, same gate arithmetic as the kernel above and as igemm16's OUT_LSTM epilogue: the same bits
 // (tests/test_gpu_bf16.py::test_convlstm_cooperative_kernel_equals_the_other_paths_bitwise, ..._keeps_two_copies_of_h under a side-stream load).
 // A block that waits ~4 s for its group (a member that never became resident) sets *err and traps: a loud failure, not a hang.
@@ -565,7 +565,7 @@ int launch_clstm16_coop(const float *zx, const void *whi, int S, int T, int rpi,
     const int rpg = (int)((cdiv((int)rows, CO_NGRP) + 31) / 32 * 32);
     const unsigned u_rpi = rpi <= 1 ? 0u : (unsigned)(((uint64_t)1 << 32) / (unsigned)rpi + 1);
     EVFLY_REQUIRE(rpi > 1, "clstm16_coop: rows per image");
-    EVFLY_HIP(hipMemsetAsync(scratch, 0, clstm16_coop_scratch_words(T) * 4, st));
+    if (int rc = fill_bytes(scratch, 0, clstm16_coop_scratch_words(T) * 4, st)) return rc;
     const float *h_in = h, *c_in = c;
     if (!fresh) {
         EVFLY_HIP(hipMemcpyAsync(state_save, h, (size_t)rows * CL_HID * 4, hipMemcpyDeviceToDevice, st));

@@ -40,6 +40,10 @@ inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s);
 // (slots may be live together on one stream).
 int scratch_get(size_t bytes, void **out, hipStream_t stream, int slot = 0);
 
+// `bytes` bytes of `value` at any device address, by a kernel: ordered and captured like every other launch. (hipMemsetAsync nodes of a captured graph
+// have been seen to give wrong results from the second replay on, and most of the callers can be captured.)
+int fill_bytes(void *dst, unsigned char value, size_t bytes, hipStream_t stream);
+
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 constexpr int kNumXCD = 8;   // MI355X: 8 XCDs, block b is observed on XCD b % 8 (speed only)

@@ -270,7 +270,7 @@ extern "C" int evfly_difflog_events(const float *im, const float *prev_im, int n
     hipStream_t st = as_stream(stream);
     void *mb = nullptr;
     if (int rc = scratch_get((size_t)n * 4, &mb, st, 0)) return rc;
-    EVFLY_HIP(hipMemsetAsync(mb, 0, (size_t)n * 4, st));
+    if (int rc = fill_bytes(mb, 0, (size_t)n * 4, st)) return rc;
     const int64_t npix = (int64_t)height * width;
     const unsigned gx = (unsigned)std::min<int64_t>((npix + 255) / 256, 1024);
     hipLaunchKernelGGL(k_difflog, dim3(gx, n), dim3(256), 0, st, im, prev_im, npix, events, static_cast<unsigned *>(mb));

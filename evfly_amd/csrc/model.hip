@@ -798,8 +798,8 @@ static int unet_chunk(evfly_model *m, const float *frames, int S, int T, float *
         if (!hs) {
             hs = m->alloc((int64_t)S * rpi * hid); cs = m->alloc((int64_t)S * rpi * hid);
             if (!m->planning) {
-                EVFLY_HIP(hipMemsetAsync(hs, 0, (size_t)S * rpi * hid * 4, st));
-                EVFLY_HIP(hipMemsetAsync(cs, 0, (size_t)S * rpi * hid * 4, st));
+                if (int rc = fill_bytes(hs, 0, (size_t)S * rpi * hid * 4, st)) return rc;
+                if (int rc = fill_bytes(cs, 0, (size_t)S * rpi * hid * 4, st)) return rc;
             }
         }
         // bf16 pipeline: the hidden-side GEMM reads a bf16 copy of h that the gate kernel keeps beside the fp32 state
@@ -994,8 +994,8 @@ static int velpred_chunk(evfly_model *m, const float *x, int S, int T, float *vp
                 EVFLY_HIP(hipMemcpy2DAsync(hs, (size_t)Hd * 4, vp_h + (int64_t)k * Hd, (size_t)c.velpred_lstm_layers * Hd * 4, (size_t)Hd * 4, S, hipMemcpyDeviceToDevice, st));
                 EVFLY_HIP(hipMemcpy2DAsync(cs, (size_t)Hd * 4, vp_c + (int64_t)k * Hd, (size_t)c.velpred_lstm_layers * Hd * 4, (size_t)Hd * 4, S, hipMemcpyDeviceToDevice, st));
             } else {
-                EVFLY_HIP(hipMemsetAsync(hs, 0, (size_t)S * Hd * 4, st));
-                EVFLY_HIP(hipMemsetAsync(cs, 0, (size_t)S * Hd * 4, st));
+                if (int rc = fill_bytes(hs, 0, (size_t)S * Hd * 4, st)) return rc;
+                if (int rc = fill_bytes(cs, 0, (size_t)S * Hd * 4, st)) return rc;
             }
         }
         for (int t = 0; t < T; ++t) {
@@ -1144,7 +1144,8 @@ static int vit_chunk(evfly_model *m, const float *img, int ih, int iw, int clip2
     // vectorised K walk -- with 48 channels it fell back to the per-element gather, 0.14 ms for 2.5 GFLOP)
     const int c_ps = c.vit_width[1] / 4, ccat_real = c_ps + c.vit_width[0], ccat = round_up(ccat_real, 32);
     float *cat = m->alloc_act((int64_t)F * 16 * 24 * ccat);
-    if (ccat != ccat_real && !m->planning) EVFLY_HIP(hipMemsetAsync(cat, 0, (size_t)F * 16 * 24 * ccat * m->esz(), st));
+    if (ccat != ccat_real && !m->planning)
+        if (int rc = fill_bytes(cat, 0, (size_t)F * 16 * 24 * ccat * m->esz(), st)) return rc;
     if (a16) {
         EVFLY_REQUIRE(c_ps % 8 == 0 && c.vit_width[0] % 8 == 0, "bf16 pipeline: ViT head widths must be multiples of 8 channels");
         RUN(m, "vit_pixel_shuffle", 0, 2 * eb * F * 384 * c_ps, launch16_pixel_shuffle2(s2, F, h2, w2, c.vit_width[1], cat, ccat, st));

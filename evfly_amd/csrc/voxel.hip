@@ -768,7 +768,8 @@ extern "C" int evfly_voxelize_windows_prepared(const uint16_t *x, const uint16_t
     // streams and the flagged frames: a 480x640 sensor at 200 k events per window needs three row bands of 4-byte cells instead of five
     // of 8-byte ones, each of which reads the whole window (C3: 3.0 -> 2.0 ms per 2560 frames).
     if (overflow) {
-        if (!overflow_cleared && !frame_first) EVFLY_HIP(hipMemsetAsync(overflow, 0, (size_t)n_frames * 4, st));      // (the frame kernel writes every frame's flag)
+        if (!overflow_cleared && !frame_first)
+            if (int rc = fill_bytes(overflow, 0, (size_t)n_frames * 4, st)) return rc;      // (the frame kernel writes every frame's flag)
         a.overflow = overflow;
     }
     if (frame_first) {
@@ -825,7 +826,7 @@ extern "C" int evfly_eventframe_rows_f64(const double *rows, int64_t n, int heig
     int32_t *counts = counts_i32 ? counts_i32 : (int32_t *)scr;
     unsigned *blk = (unsigned *)((char *)scr + counts_bytes);
     unsigned long long *total = (unsigned long long *)((char *)scr + counts_bytes + blk_bytes);
-    EVFLY_HIP(hipMemsetAsync(counts, 0, (size_t)2 * hw * 4, st));
+    if (int rc = fill_bytes(counts, 0, (size_t)2 * hw * 4, st)) return rc;
     if (n > 0) {
         if (mode == 1) {
             hipLaunchKernelGGL(k_rows_count, dim3(n_blocks), dim3(kRowsThreads), 0, st, rows, n, t0_ns, blk);
@@ -850,7 +851,7 @@ extern "C" int evfly_eventframe_rows_f64(const double *rows, int64_t n, int heig
 
 extern "C" int evfly_accumulate_reset(uint8_t *img, int64_t n_pixels, void *stream) {
     EVFLY_REQUIRE(img && n_pixels > 0, "accumulate_reset: empty image");
-    EVFLY_HIP(hipMemsetAsync(img, 128, (size_t)n_pixels, as_stream(stream)));   // node.cpp:10,58
+    if (int rc = fill_bytes(img, 128, (size_t)n_pixels, as_stream(stream))) return rc;   // node.cpp:10,58
     return 0;
 }
 
@@ -867,8 +868,8 @@ extern "C" int evfly_accumulate_u8(const uint16_t *x, const uint16_t *y, const u
     unsigned *on = (unsigned *)scr, *off = (unsigned *)((char *)scr + plane);
     int *hot_list = (int *)((char *)scr + 2 * plane);
     int *hot_count = (int *)((char *)scr + 3 * plane);
-    EVFLY_HIP(hipMemsetAsync(scr, 0, 2 * plane, st));
-    EVFLY_HIP(hipMemsetAsync(hot_count, 0, 4, st));
+    if (int rc = fill_bytes(scr, 0, 2 * plane, st)) return rc;
+    if (int rc = fill_bytes(hot_count, 0, 4, st)) return rc;
     const int blocks = (int)std::min<int64_t>(4 * kNumCU, cdiv(n, 256));
     hipLaunchKernelGGL(k_acc_count, dim3(blocks), dim3(256), 0, st, x, y, polarity, n, width, height, on, off);
     hipLaunchKernelGGL(k_acc_apply, dim3(cdiv(n_pix, 256)), dim3(256), 0, st, img, n_pix, mode, on, off, hot_list,

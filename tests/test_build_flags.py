@@ -19,3 +19,10 @@ def test_no_source_spells_packed_fp32():
     for path in glob.glob(os.path.join(CSRC, "*.h*")):
         for i, line in enumerate(open(path), 1):
             assert not re.search(r"v_pk_(add|mul|fma)_f32", line), f"{path}:{i}"
+
+
+def test_no_source_queues_a_memset():
+    """A captured hipMemsetAsync node may go wrong on replays: memory is filled by a kernel."""
+    for path in glob.glob(os.path.join(CSRC, "*.h*")):
+        code = re.sub(r"//[^\n]*", "", open(path).read())
+        assert "hipMemsetAsync" not in code, path
