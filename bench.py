@@ -48,12 +48,9 @@ PMC_TRAFFIC = {"C2": ("r6_C2_pmc_traffic.json", "r5_C2_pmc_traffic.json", "r4_C2
                "C5": ("r6_C5_pmc_traffic.json", "r5_C5_pmc_traffic.json", "r4_C5_pmc_traffic.json"), "C3": ("r6_C3_pmc_traffic.json", "r5_C3_pmc_traffic.json")}
 
 CONFIGS = {
-    # The composite configs run the velocity model on a second HIP stream (evfly_amd/pipeline.py; --no-overlap: one stream). With the
-    # ViT-base trunk in bf16 (C3) it is a third of the step and made of launches that leave most of the chip idle (80.2 -> 76.1 ms per
-    # step when it was introduced). With the fp32 Winograd kernels holding every CU's LDS the gain is small but repeatable -- C2 same box,
-    # three alternating runs: 21.11 / 21.12 / 21.13 -> 20.91 / 20.88 / 20.86 ms (+ 1.2 %) -- and kernels of two streams sharing the chip stretch
-    # the HIP-event durations the roofline is computed from (`frac` 0.661 -> 0.644 inside the timed region): the line carries
-    # `roofline.one_stream`, the same family over three one-stream steps outside the timed region, beside it.
+    # The composite configs run the velocity model over all of a step's frames on a second HIP stream, behind the depth model and in front of the next
+    # step (evfly_amd/pipeline.py; --no-overlap: the composite call, whose velocity model runs per chunk of the depth model). The two models do not
+    # share the chip. `roofline.one_stream` beside the timed region's figures: the same family over three one-stream steps.
     "C2": dict(streams=64, windows=5, epw=60_000, sensor=(260, 346), vit="tiny", dtype="f32", model="composite", overlap=True),
     "C3": dict(streams=256, windows=10, epw=200_000, sensor=(480, 640), vit="base", dtype="bf16", model="composite", overlap=True),
     "C4": dict(streams=256, windows=5, epw=60_000, sensor=(260, 346), vit="base", dtype="f32", model="composite", overlap=True),
@@ -75,10 +72,10 @@ def parse():
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-alt", action="store_true", help="skip the informational bf16x3 pass (C2 only)")
     ap.add_argument("--no-other-configs", action="store_true", help="default C2 run: skip the compact C5 / C3 / C4 objects")
-    ap.add_argument("--no-overlap", action="store_true", help="run the velocity model back to back behind the depth model on one "
-                    "stream (the composite call) even where the config's default is the two-stream pipeline (C3)")
-    ap.add_argument("--overlap", action="store_true", help="velocity model of step i on a second HIP stream under the depth model "
-                    "of step i + 1 (evfly_amd/pipeline.py) for every composite config")
+    ap.add_argument("--no-overlap", action="store_true", help="one stream and the composite call, even where the config's "
+                    "default is the pipeline of two streams")
+    ap.add_argument("--overlap", action="store_true", help="velocity model on a second HIP stream between the depth models of "
+                    "step i and step i + 1 (evfly_amd/pipeline.py) for every composite config")
     ap.add_argument("--no-stage-rates", action="store_true", help="skip the V / D / P-only timings")
     ap.add_argument("--pmc-pass", action="store_true", help="shape of a rocprofv3 --pmc counter pass: ONE stream, nothing but whole steps "
                     "(warm-up + one bracketed + K timed; no stage timings, no one-stream probe, no side configs), so that every kernel's "
@@ -346,10 +343,8 @@ def run_config(a, cname, cfg, rank, world, dist, detail):
     frames = torch.empty(B, T, H, W, device="cuda")
     counts = shard_row_counts(world * B, world, T)                                  # every rank: B streams (weak scaling)
     vel_host = torch.empty(world * B * T, 3).pin_memory() if composite else None    # §8d: "velocity rows on host-visible memory"
-    # Two-stream pipeline (evfly_amd/pipeline.py): the velocity model of step i (ViT + LSTM, ~55 small launches) runs on a second HIP
-    # stream behind the depth model's completion event while the first stream goes on with voxelize + condition + depth model of
-    # step i + 1 -- the same kernels and bits as the back-to-back composite call, the small launches filling the large ones' gaps.
-    # The timed region still closes with a device-wide synchronize: all K steps' velocities are in pinned host memory inside it.
+    # Pipeline of two streams (evfly_amd/pipeline.py): the velocity model of step i (ViT + LSTM, ~55 small launches), its all_gather and its copy to
+    # the host on a second HIP stream between the depth models of steps i and i + 1 -- the same kernels and bits as the composite call. The timed region still closes with a device-wide synchronize: all K steps' velocities are in pinned host memory inside it.
     pipe = None
     if composite and not a.no_overlap and (a.overlap or cfg.get("overlap")):
         from evfly_amd.pipeline import StreamPipeline
@@ -433,8 +428,7 @@ def run_config(a, cname, cfg, rank, world, dist, detail):
     timed_rec = bracketed()
     one_stream = None
     if pipe:
-        # the same steps on ONE stream, outside the timed region: in the timed region kernels of the two streams share the chip, which
-        # stretches the HIP-event durations of the dominant family; this pass times the family alone (3 steps)
+        # the same steps on ONE stream, outside the timed region (3 steps)
         def step_serial():
             calls[0] += 1
             voxelizer.voxelize_windows(ev, Hs, Ws, out="f32", frames=frames, roi=roi)
@@ -535,7 +529,7 @@ def run_config(a, cname, cfg, rank, world, dist, detail):
                    "streams_per_gpu": B, "windows": T, "events_per_step_per_gpu": n_events, "sensor": [Hs, Ws], "vit_trunk": cfg["vit"] if composite else None,
                    "parallelism": f"streams sharded x{world}, all_gather of velocities" if world > 1 else "single GPU"},
         "step_ms": step_ms, "steps_executed": calls[0],
-        "pipeline": ("two HIP streams: velocity model (ViT + LSTM) of step i under voxelize + depth model of step i + 1 "
+        "pipeline": ("two HIP streams: velocity model (ViT + LSTM) of step i behind its depth model, step i + 1 behind both "
                      "(evfly_amd/pipeline.py; --no-overlap = one stream)" if pipe else "one HIP stream"),
     }
     if dist is not None:

@@ -1,12 +1,13 @@
-"""Two-stream throughput mode of the composite D(theta) -> V(phi) (learner/learner_models.py:618-636).
+"""A stream of batches through the composite D(theta) -> V(phi) (learner/learner_models.py:618-636), the velocity model on a stream of its own.
 
-`OrigUNet_w_VITFLY_ViTLSTM.forward` runs the depth model and the velocity model back to back, as the reference does. For a
-STREAM of batches (evfly_ros/run.py:245-268 called at 15 Hz per camera; bench.py's steps) the two models only meet at the depth
-image: D of batch i + 1 needs nothing from P of batch i (the ConvLSTM state goes D -> D, the nn.LSTM state P -> P). `StreamPipeline`
-therefore launches P(i) on a second HIP stream behind an event and lets the caller's stream go on with V + D of batch i + 1: the
-velocity model's ~55 small, latency-shaped launches (1.5 ms per 320 frames at 23 TFLOP/s) fill the gaps and kernel tails of the
-depth model's large launches instead of running alone on an idle chip. Same kernels, same order inside each model, same bits as
-the composite call (tests/test_gpu_models.py::test_stream_pipeline_equals_composite).
+`OrigUNet_w_VITFLY_ViTLSTM.forward` is one call per batch, as in the reference. For a STREAM of batches (evfly_ros/run.py:245-268 called at 15 Hz per
+camera; bench.py's steps) `StreamPipeline` queues the two models separately, their states kept apart (the ConvLSTM state goes D -> D, the nn.LSTM state
+P -> P): D on the caller's stream, P and what follows it (the all_gather, the copy to pinned host memory) on a second HIP stream behind D's event, and the
+caller's stream behind P's. Same kernels, same order, same bits as the composite call (tests/test_gpu_models.py::test_stream_pipeline_equals_composite).
+
+The two models do not share the device. Nothing of D(i + 1) needs P(i), but run together they have not been sound: with the bf16 U-Net of 2560 frames and
+the ViT-base trunk, 2 to 5 % of the steps whose depth model ran beside a velocity model had wrong depth in the first frames of their second chunk, the
+same steps one after the other never. The cause was not found in the kernels; the overlap was worth 1 to 2 %.
 
 No reference counterpart beyond the call pattern above: the reference is single-stream PyTorch.
 """
@@ -24,41 +25,29 @@ class StreamPipeline:
         self.unet.set_compute_dtype(name)           # (the setter also thaws a frozen handle: a plain attribute write does not)
         self.vit.set_compute_dtype(name)
         self.side = torch.cuda.Stream()
-        self._done = None
-        self._side_tensors = []
 
     def step(self, frames, desvel, n_streams, T, unet_state=None, vit_state=None, after=None):
-        """One batch, laid out [stream][t] like `forward_streams`. D runs on the current stream; P is queued on the side stream
-        behind D's completion event and `after(vel)` (e.g. the all_gather + copy to pinned host memory) right behind it, still on
-        the side stream. Returns (vel, (depth, upconv, ((h_unet, None), (lstm_h, lstm_c))), after's result): `vel` and the LSTM
-        state are valid once `wait()` (or a device synchronize) has returned; depth / upconv / h_unet on the current stream."""
+        """One batch, laid out [stream][t] like `forward_streams`. D runs on the current stream, P on the side stream behind it, then `after(vel)` (e.g. the
+        all_gather + copy to pinned host memory), still on the side stream; the current stream goes on behind them. Returns
+        (vel, (depth, upconv, ((h_unet, None), (lstm_h, lstm_c))), after's result), all valid on the current stream."""
         depth, upconv, h_unet = self.unet.forward_streams(frames, unet_state, n_streams, T)
-        ev = torch.cuda.Event()
-        ev.record()
         main = torch.cuda.current_stream()
+        self.side.wait_stream(main)
         with torch.cuda.stream(self.side):
-            self.side.wait_event(ev)
             depth.record_stream(self.side)                 # the caching allocator must not recycle it under P
             X = [depth, desvel, None] + ([vit_state] if vit_state is not None else [])
             vel, st = self.vit._run(X, n_streams, T, clip2x=1)      # x_depth_input = clip(2 * depth, 0, 1), learner_models.py:634
             extra = after(vel) if after is not None else None
-            self._done = torch.cuda.Event()
-            self._done.record()
-        # vel, the LSTM state and after's result were allocated from the SIDE stream's pool of the caching allocator: `wait()` hands them to
-        # the waiting stream (record_stream), otherwise a consumer on that stream could still be reading a block that the allocator has
-        # already given to the next step's velocity model on the side stream
-        self._side_tensors = [t for t in _flatten((vel, st, extra)) if isinstance(t, torch.Tensor) and t.is_cuda]
-        del main
+        main.wait_stream(self.side)
+        # vel, the LSTM state and after's result come from the SIDE stream's pool of the caching allocator: their readers are on this stream
+        for t in _flatten((vel, st, extra)):
+            if isinstance(t, torch.Tensor) and t.is_cuda:
+                t.record_stream(main)
         return vel, (depth, upconv, ((h_unet, None), st)), extra
 
     def wait(self):
-        """Make the current stream wait for everything queued on the side stream so far; the tensors the last step produced there
-        (vel, the LSTM state, `after`'s result) may then be used -- and dropped -- on the current stream."""
-        if self._done is not None:
-            cur = torch.cuda.current_stream()
-            cur.wait_event(self._done)
-            for t in self._side_tensors:
-                t.record_stream(cur)
+        """The results of `step` are ordered on the stream that it was called on; a reader on another stream waits for that one."""
+        torch.cuda.current_stream().wait_stream(self.side)
 
 
 def _flatten(x):
