@@ -539,8 +539,8 @@ struct BnPlan {
     unsigned blocks;
     int64_t o_gate, bytes;
 };
-// Backward: units of rows that share a gate row. One gate row for everything (or none, or one per row): about two units per block so that the blocks end
-// together; a gate row per stream: enough parts of each stream that every block has work, at least two rows per group each.
+// Backward: units of rows that share a gate row. One gate row for everything (or none, or one per row): one unit per block, of equal rows; a gate row
+// per stream: enough parts of each stream that every block has work. At least two rows per group in either.
 BnPlan bn_plan(int64_t rows, int C, int64_t rpg) {
     BnPlan b{};
     b.G = lanes_for(C);

@@ -270,10 +270,11 @@ void token_strides(const int64_t *s, int T, int heads, int d, int64_t (&out)[3])
 // pass, 0.4 of a chunk's work) and adds two launches. The split with the smallest estimate, in us, is taken:
 //     (chunks per segment + 1/2) * t * max(1, share * blocks per CU)      for each launch of the pass and, at 0.4 t, for the state pass
 //     + 5 + 0.15 * segments                                               if it is cut at all (the scan over the borders)
-// with t the time of a lone block's chunk (by type and a dimension) and `share` what a block uses of its CU. Against sweeps of 1 .. 64 segments on thirteen shapes, forward and
-// backward, the choice is within 10 % of the best; us forward / backward, chosen and neighbours: 8 x 4096 tokens x 16 heads x 64 bf16, four 99 forward (two 133,
-// eight 104), two 198 backward (one 219, four 218); 1 x 16384 x 4 x 64 bf16, 64 segments 49 forward (16: 75); 1 x 32768 x 16 x 128 bf16, 16 segments 258 (8: 330, 32: 270); 6 x
-// 500 x 8 x 40 / 72 fp32, eight 33 / 82 (four 37 / 89, one 52 / 129); 16 x 1000 x 8 x 32 bf16, four 25 forward (one 27), one 33 backward (two 37).
+// with t the time of a lone block's chunk (by type and a dimension) and `share` what a block uses of its CU. It ranks the splits, it does not tell their times (30 and 317 where 49 and
+// 276 are measured). Against sweeps of 1 .. 64 segments on thirteen shapes, forward and backward (profiles/temporal_segments.txt), the choice is within 4 % of the best in 24
+// of 26 and 11 and 15 % off in two; us forward / backward, chosen and neighbours: 8 x 4096 tokens x 16 heads x 64 bf16, four 100 forward (two 133, eight 110), two 212
+// backward (one 228, four 219); 1 x 16384 x 4 x 64 bf16, 64 segments 49 forward (16: 73); 1 x 32768 x 16 x 128 bf16, 16 segments 271-281 (8: 372, 32: 288); 6 x
+// 500 x 8 x 40 / 72 fp32, eight 33 / 84 (four 37 / 90, one 53 / 131); 16 x 1000 x 8 x 32 bf16, four 26 forward (one 30), one 36 backward (two 40).
 namespace {
 int col_tiles(int c) { return (c + decay_tile_c(c) - 1) / decay_tile_c(c); }
 // the gradients' passes have their roles exchanged: one launch serves all three if both head sizes have the same tiles

@@ -26,6 +26,7 @@ _GATE_ACT = {a: _lib.ACT_CODES[a] for a in ("none", "sigmoid", "tanh")}
 
 
 _getDevice, _rawStream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream      # (a tick's call is a few microseconds: no Stream object for it)
+_tracingState, _dispatchModes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
 
 
 def _ptr(t):
@@ -40,14 +41,19 @@ def _workspace(nbytes, like):
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes > 0 else None
 
 
+def _watched():
+    """Something other than autograd may follow the call (`_refuse_unseen`)."""
+    return _forward_ad._current_level >= 0 or _dispatchModes() > 0 or _tracingState() is not None
+
+
 def _refuse_unseen(who, tensors, recorded):
     """The library's work is no torch operation: forward-mode differentiation takes its results for constants, a tracer for memory that nothing writes. (recorded: the
     call is an autograd function's, which torch.jit.trace keeps as a whole.)"""
     if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{who} has no forward-mode derivatives")
-    if not recorded and torch._C._get_tracing_state() is not None:
+    if not recorded and _tracingState() is not None:
         raise RuntimeError(f"{who}: torch.jit.trace does not see its work")
-    if torch._C._len_torch_dispatch_stack() > 0:
+    if _dispatchModes() > 0:
         from torch.fx.experimental.proxy_tensor import get_proxy_mode
         if get_proxy_mode() is not None:
             raise RuntimeError(f"{who}: make_fx does not see its work")
@@ -222,7 +228,8 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     scale: dk ** -0.5 if None. Returns (out (streams, tokens, heads, dv), new state). Gradients to q, k, v and state."""
     scale = _check_decay("decay_attention", q, k, v, log_decay, state, lengths, scale, 2)
     recorded = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad))
-    _refuse_unseen("decay_attention", (q, k, v, log_decay, state), recorded)
+    if _watched():
+        _refuse_unseen("decay_attention", (q, k, v, log_decay, state), recorded)
     if recorded:
         return _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale)
     new_state = _new_state(q, v)
@@ -243,12 +250,14 @@ def decay_attention_step(q, k, v, log_decay, state, lengths=None, scale=None, ne
         _check_f32(who, "new_state", new_state, state.shape, q.device)
         if not new_state.is_contiguous():
             raise ValueError(f"{who}: new_state must be a contiguous tensor")
-        if 0 < abs(new_state.data_ptr() - state.data_ptr()) < 4 * state.numel():
+        apart = new_state.data_ptr() - state.data_ptr()
+        if apart and abs(apart) < 4 * state.numel():
             raise ValueError(f"{who}: state and new_state overlap in part")
         dst = new_state
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or dst.requires_grad):
         raise ValueError(f"{who} has no gradients: call decay_attention, or wrap the call in torch.no_grad()")
-    _refuse_unseen(who, (q, k, v, log_decay, state, new_state), False)
+    if _watched():
+        _refuse_unseen(who, (q, k, v, log_decay, state, new_state), False)
     out = _decay_forward(q, k, v, log_decay, state, lengths, scale, dst)
     if not dst.is_inference():                                   # (an inference tensor has no version)
         torch.autograd.graph.increment_version(dst)              # written behind autograd's back
@@ -398,7 +407,8 @@ def block_norm(f, x=None, gate=None, gate_act="none", res_scale=None, post=None,
             if t is not None and t.requires_grad:
                 recorded = True
                 break
-    _refuse_unseen("block_norm", ins, recorded)
+    if _watched():
+        _refuse_unseen("block_norm", ins, recorded)
     if recorded:
         got = _BlockNorm.apply(*ins, opt)
         return got if isinstance(got, tuple) else (got, None)
