@@ -182,9 +182,10 @@ template <typename T> __global__ __launch_bounds__(256) void k_decay_head_sum(He
     }
 }
 
-// The recurrence costs a step per token, a chunk of 64 the same for one token as for all. Forward, us, recurrence against chunk: 256 streams x 8 heads x 64, bf16, 8
-// tokens 18 / 23, 12 tokens 25 / 23; 64 x 16 x 128, bf16, 12 tokens 39 / 43, 16 tokens 50 / 43; 256 x 8 x 32, bf16, 16 tokens 15.4 / 15.6; fp32, 256 x 8 x 64, 16 tokens
-// 31 / 39; 64 x 16 x 128, 16 tokens 51 / 113.
+// The recurrence costs a step per token, a chunk of 64 the same for one token as for all. Forward, us, recurrence against chunk, bf16: 256 streams x 8 heads x 64, 8 tokens
+// 20 / 28, 11 tokens 24 / 28, 13 tokens 28 / 28; 16 x 8 x 128, 11 tokens 13.6 / 13.5, 16 tokens 17 / 13.5; 64 x 16 x 128, 12 tokens 45 / 52, 16 tokens 54 / 51. So the
+// crossing lies between 11 and 16 tokens, earliest where few blocks run; from 11 on the side not taken is up to a fifth better on large batches. 256 x 8 x 32, bf16, 16 tokens
+// 15.0 / 15.9; fp32, 16 tokens, 256 x 8 x 64 32 / 34, 64 x 16 x 128 56 / 106, 16 x 8 x 128 16.7 / 16.4.
 bool recurrent(int tokens, int dk, int dv, int dtype) {
     const bool quick_chunk = dtype == EVFLY_DTYPE_BF16 && (dk > 32 || dv > 32);
     return tokens <= (quick_chunk ? 11 : EVFLY_DECAY_STEP_TOKENS);

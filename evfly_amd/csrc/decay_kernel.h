@@ -11,9 +11,9 @@
 // the state's a-rows. The a rows go from memory to the wave's registers, b and c through LDS (read as rows for P, as columns for the other two
 // products), S lives in the accumulators and is copied to LDS once per chunk as an operand of a_i S. The next chunk's rows are in flight during the products.
 //
-// Bounds. bf16, 64 wide (8 x 4096 tokens x 16 heads): a pass moves 268 MB in 70 us, 3.8 TB/s of the 4.9 that a copy reaches here. bf16, 128 wide
-// (1 x 32768 x 16): 178 us; counted busy are the matrix pipes 31 %, vector issue 52 %, LDS 53 % of the time: two waves per SIMD (61 KB of LDS a block)
-// overlap them only in part. fp32: the 16x16x4 products, 43 % of their pipe's time at 48 / 96 wide with two blocks a CU.
+// Bounds (medians under the profiler). bf16, 64 wide (8 x 4096 tokens x 16 heads): a pass moves 268 MB in 76 us, 3.5 TB/s of the 4.9 that a copy reaches here. bf16,
+// 128 wide (1 x 32768 x 16): 220 us; counted busy are the matrix pipes 35 %, vector issue 57 %, LDS 61 % of the time (46 % of its cycles conflicts): two waves per SIMD
+// (78 KB of LDS a block, 51 of them the state's three parts) overlap them only in part. fp32: the 16x16x4 products, 45 % of their pipe's time at 48 / 96 wide with two blocks a CU.
 #pragma once
 #include "bf16.h"
 #include "decay.h"
@@ -144,7 +144,7 @@ template <typename T, int DA, int DC, bool STATE> constexpr int blocks_per_cu() 
 }
 
 // STATE: the segment's own state only (no output), for the sequences that are split into segments. TAIL: a head size that is no whole number of 16-byte
-// pieces (without it the loop is free of the branches of partial pieces: 8 x 4096 x 16 heads x 64, bf16, 70 us a pass against 76).
+// pieces (without it the loop is free of the branches of partial pieces: 8 x 4096 x 16 heads x 64, bf16, measured with two parts a value: 70 us a pass against 76).
 template <typename T, int DA, int DC, bool STATE, bool TAIL>
 __global__ __launch_bounds__(256, (blocks_per_cu<T, DA, DC, STATE>())) void k_decay_chunk(DecayPasses ps) {
     typedef Mm<T> M;
