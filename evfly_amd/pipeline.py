@@ -30,15 +30,18 @@ class StreamPipeline:
         """One batch, laid out [stream][t] like `forward_streams`. D runs on the current stream, P on the side stream behind it, then `after(vel)` (e.g. the
         all_gather + copy to pinned host memory), still on the side stream; the current stream goes on behind them. Returns
         (vel, (depth, upconv, ((h_unet, None), (lstm_h, lstm_c))), after's result), all valid on the current stream."""
-        depth, upconv, h_unet = self.unet.forward_streams(frames, unet_state, n_streams, T)
         main = torch.cuda.current_stream()
+        main.wait_stream(self.side)                        # (a step before this one may have been another stream's)
+        depth, upconv, h_unet = self.unet.forward_streams(frames, unet_state, n_streams, T)
         self.side.wait_stream(main)
-        with torch.cuda.stream(self.side):
-            depth.record_stream(self.side)                 # the caching allocator must not recycle it under P
-            X = [depth, desvel, None] + ([vit_state] if vit_state is not None else [])
-            vel, st = self.vit._run(X, n_streams, T, clip2x=1)      # x_depth_input = clip(2 * depth, 0, 1), learner_models.py:634
-            extra = after(vel) if after is not None else None
-        main.wait_stream(self.side)
+        try:
+            with torch.cuda.stream(self.side):
+                depth.record_stream(self.side)             # the caching allocator must not recycle it under P
+                X = [depth, desvel, None] + ([vit_state] if vit_state is not None else [])
+                vel, st = self.vit._run(X, n_streams, T, clip2x=1)  # x_depth_input = clip(2 * depth, 0, 1), learner_models.py:634
+                extra = after(vel) if after is not None else None
+        finally:
+            main.wait_stream(self.side)                    # (also where `after` raises: P is under way by then)
         # vel, the LSTM state and after's result come from the SIDE stream's pool of the caching allocator: their readers are on this stream
         for t in _flatten((vel, st, extra)):
             if isinstance(t, torch.Tensor) and t.is_cuda:
