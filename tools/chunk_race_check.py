@@ -4,7 +4,7 @@
 
 Runs the composite's two halves (depth model, velocity model) of a bf16 ViT-base handle pair on random conditioned frames
   (a) twice on one stream (bitwise reproducible?),
-  (b) three pipelined steps (velocity model of step i on the side stream under the depth model of step i + 1),
+  (b) three pipelined steps (velocity model of step i on the side stream, in front of the depth model of step i + 1),
 and prints which of them differ, per 320-frame block of velocity rows.
 """
 import os

@@ -1,6 +1,6 @@
 """Do the velocity head's kernels (ViT + LSTM: small, latency / HBM bound) hide under the U-Net's (Winograd: matrix-pipe bound) when
 the two run on different HIP streams? Times D alone, P alone, D then P on one stream, D || P on two streams (half batches, the
-pipelined composite a two-chunk schedule would give).  usage: python tools/overlap_probe.py [streams]"""
+pipelined composite a two-chunk schedule would give). Times only: the package does not run the two together, see evfly_amd/pipeline.py.  usage: python tools/overlap_probe.py [streams]"""
 import sys, os
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch
